@@ -22,7 +22,7 @@ import torch
 own = False
 
 BLOCK = 128
-EPS = 1e-6
+EPS = 2.0 ** -20  # (a number of f32, which is what the operator takes)
 ALPHA, ADAM_EPS, B1, B2 = 1e-3, 1e-8, 0.9, 0.999
 # gradients of the small convolutional net's parameters (filters, dense layer and biases of its three layers)
 SMALL_NET = (32 * 9, 64 * 32 * 9, 3136 * 10, 32 * 28 * 28, 64 * 14 * 14, 10)
@@ -152,7 +152,7 @@ def prepare(case, seed):
 # ---- the plain form --------------------------------------------------------------------------------------------------
 def _quantize(x):
     """x [rows, n] -> (q, scales) in the layout above.  The scale of a block is the smallest power of two, at least
-    2^-126, that brings the block's largest finite magnitude to at most 448; a block of zeros has scale 1.  Values that
+    2^-117, that brings the block's largest finite magnitude to at most 448; a block of zeros has scale 1.  Values that
     are not finite become NaN."""
     rows, n = x.shape
     blocks = -(-n // BLOCK)
@@ -163,7 +163,7 @@ def _quantize(x):
     amax = torch.where(finite, padded.abs(), torch.zeros_like(padded)).amax(2)
     mantissa, exponent = torch.frexp(amax.double())  # amax = mantissa * 2^exponent, mantissa in [1/2, 1)
     byte = exponent - 9 + (mantissa > 0.875).int() + 127  # 448 = 0.875 * 2^9
-    byte = torch.where(amax > 0, byte.clamp(min=1), torch.full_like(byte, 127)).int()
+    byte = torch.where(amax > 0, byte.clamp(min=10), torch.full_like(byte, 127)).int()
     inverse = ((254 - byte) << 23).view(torch.float32)  # 2^(127 - byte), by its bits
     scaled = padded * inverse[:, :, None]
     q = torch.where(finite, scaled, torch.full_like(scaled, math.nan)).to(torch.float8_e4m3fn)
@@ -323,7 +323,7 @@ def _exact_rounded(x, layout=False):
     v = torch.nn.functional.pad(x.double(), (0, blocks * BLOCK - n)).view(rows, blocks, BLOCK)
     top = v.abs().amax(2).float().view(torch.int32)  # exact: the inputs are f32
     e = (top >> 23) - 127 - 8 + ((top & 0x7FFFFF) > 0x600000).int()
-    e = torch.where(top > 0, e.clamp(min=-126), torch.zeros_like(e)).long()
+    e = torch.where(top > 0, e.clamp(min=-117), torch.zeros_like(e)).long()
     scale = ((e + 1023) << 52).view(torch.float64)[:, :, None]
     v = v / scale
     _, k = torch.frexp(v)
