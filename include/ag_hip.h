@@ -373,6 +373,80 @@ ag_status_t ag_sparse_softmax_xent_grad_logits_f32(ag_stream_t stream, const flo
                                                    float gy_const, float *gx, size_t rows,
                                                    size_t classes);
 
+/* ---- 8-bit operands and their product --------------------------------------------------------- */
+
+/* An 8-bit operand of `rows` rows and n elements along the contraction is
+ *   q      [rows, ag_e4m3_pitch(n)]        one e4m3 byte per element (1 sign, 4 exponent and 3 mantissa bits, largest
+ *                                          value 448, no infinities), rows padded with zeros to a multiple of 128;
+ *   scales [rows, ag_e4m3_scale_pitch(n)]  one byte b per block of 128 elements, which stands for the factor 2^(b-127);
+ *                                          the number of blocks rounded up to 4, the rest 127 (a factor of one).
+ * An element's value is q * scale.  No counterpart in the reference, whose arrays are f32 or f64. */
+size_t ag_e4m3_pitch(int n);
+size_t ag_e4m3_scale_pitch(int n);
+
+/* Rounds x [rows, cols] (row stride ldx) to such operands: along its rows into q, scales, along its columns into qt
+ * [cols, ag_e4m3_pitch(rows)] and scales_t (the transposed array); either pair may be NULL, one pass over x serves both.
+ * The scale of a block is the smallest power of two, at least 2^-117, with the block's largest finite magnitude at most
+ * 448 times it (1 for a block of zeros); elements are rounded to nearest, ties to even.  An element that is not finite
+ * becomes NaN and takes no part in the scale.  q and qt are 16-byte aligned. */
+ag_status_t ag_quantize_e4m3_f32(ag_stream_t stream, const float *x, int ldx, int rows, int cols, uint8_t *q,
+                                 uint8_t *scales, uint8_t *qt, uint8_t *scales_t);
+
+/* C[M x N] = A . B^T of the 8-bit operands A (M rows) and B (N rows), K elements along the contraction, f32 accumulation
+ * and output, row stride ldc.  Each product of two blocks is exact; sums are f32 in an order that depends on the extents
+ * only.  A NaN reaches the elements that it takes part in.  With a [M,K], b [K,N] and y = a . b, and each operand rounded
+ * along the contraction it enters: y = (a along rows) (b along columns), ga = (gy along rows) (b along rows),
+ * gb = (a along columns) (gy along columns).  A and B are 16-byte aligned, their scales 4-byte aligned; K is at most 2^28.
+ * ws: ag_matmul_e4m3_f32_workspace() bytes, 16-byte aligned. */
+size_t ag_matmul_e4m3_f32_workspace(int M, int N, int K);
+ag_status_t ag_matmul_e4m3_f32(ag_stream_t stream, int M, int N, int K, const uint8_t *A, const uint8_t *a_scales,
+                               const uint8_t *B, const uint8_t *b_scales, float *C, int ldc, void *ws, size_t ws_bytes);
+
+/* The same product with the left operand given in f32: x [M,K] (row stride ldx) is rounded as ag_quantize_e4m3_f32
+ * rounds along rows, with the same bits, and multiplied by B in one call: a layer whose weight was laid out in 8 bits
+ * once.  ws: ag_quantize_matmul_e4m3_f32_workspace() bytes, 16-byte aligned. */
+size_t ag_quantize_matmul_e4m3_f32_workspace(int M, int N, int K);
+ag_status_t ag_quantize_matmul_e4m3_f32(ag_stream_t stream, int M, int N, int K, const float *x, int ldx, const uint8_t *B,
+                                        const uint8_t *b_scales, float *C, int ldc, void *ws, size_t ws_bytes);
+
+/* ---- root-mean-square norm -------------------------------------------------------------------- */
+
+/* Rows of n elements: h = x + residual, y = h * weight / sqrt(mean(h^2) + eps), the statistics and y in 64 bits, y
+ * rounded to f32 once.  Outputs, each may be NULL: h and y [rows, n] f32; q, scales: y rounded along its rows as
+ * ag_quantize_e4m3_f32 does (same bits); rstd [rows], 1 / sqrt(mean(h^2) + eps) in f32, which the gradient reads.
+ * residual may be NULL (h is then a copy of x).  h and y may be the arrays x and residual, not the same one. */
+ag_status_t ag_rms_norm_f32(ag_stream_t stream, const float *x, const float *residual, const float *weight, float eps,
+                            float *h, float *y, uint8_t *q, uint8_t *scales, float *rstd, int rows, int n);
+
+/* Its gradient: gx = rstd * weight * gy - h * rstd^3 / n * sum(weight * gy * h) (+ gh, the gradient that reaches h on
+ * other ways; may be NULL), which is that of x and of residual, and gw [n] = sum over rows of gy * h * rstd, added in an
+ * order that depends on the extents only.  gx or gw may be NULL; gx may be the array gy or gh.  ws (for gw):
+ * ag_rms_norm_grad_f32_workspace() bytes. */
+size_t ag_rms_norm_grad_f32_workspace(int rows, int n);
+ag_status_t ag_rms_norm_grad_f32(ag_stream_t stream, const float *h, const float *weight, const float *rstd,
+                                 const float *gy, const float *gh, float *gx, float *gw, int rows, int n, void *ws,
+                                 size_t ws_bytes);
+
+/* ---- norm over all gradients, and clipping by it ----------------------------------------------- */
+
+/* clip[0] = sqrt(sum of the squares of all elements of `count` arrays), clip[1] = clip[0] <= max_norm ? 1 :
+ * max_norm / clip[0]: two floats in device memory.  Squares are added in 64 bits in a fixed order.  A NaN among the
+ * elements makes both NaN; an infinity makes the coefficient 0.  xs, ns: host tables, read before the call returns.  ws:
+ * ag_global_norm_f32_workspace() bytes, 8-byte aligned. */
+size_t ag_global_norm_f32_workspace(int count, const size_t *ns);
+ag_status_t ag_global_norm_f32(ag_stream_t stream, int count, const float *const *xs, const size_t *ns, float max_norm,
+                               float *clip, void *ws, size_t ws_bytes);
+/* That, followed by outs[i] = xs[i] * clip[1].  outs[i] is xs[i] or overlaps no array of the call
+ * (AG_ERR_INVALID_DIMS). */
+ag_status_t ag_clip_by_global_norm_f32(ag_stream_t stream, int count, const float *const *xs, float *const *outs,
+                                       const size_t *ns, float max_norm, float *clip, void *ws, size_t ws_bytes);
+/* ag_adam_update_multi_f32 with every gradient multiplied by clip[1] (device memory, as ag_global_norm_f32 writes it)
+ * where the update reads it: the bits of clipping first, without the pass over the gradients. */
+ag_status_t ag_adam_update_multi_clipped_f32(ag_stream_t stream, int count, float *const *params,
+                                             const float *const *grads, float *const *ms, float *const *vs,
+                                             float *const *ts, const size_t *ns, float alpha, float eps, float b1,
+                                             float b2, const float *clip);
+
 /* ---- entry point that allocates nothing ----------------------------------------------------- */
 
 /* ag_matmul_f32 without a workspace argument.  No counterpart in the reference: it is for callers

@@ -110,6 +110,20 @@ PROTOTYPES = {
     "ag_conv2d_nocols_with_filter_f32": (c_i, [c_p, c_p, c_p, c_p, c_p] + [c_i] * 10),
     "ag_conv2d_filter_grad_nocols_f32_workspace": (c_sz, [c_i] * 10),
     "ag_conv2d_filter_grad_nocols_f32": (c_i, [c_p, c_p, c_p, c_p] + [c_i] * 10 + [c_p, c_sz]),
+    "ag_e4m3_pitch": (c_sz, [c_i]),
+    "ag_e4m3_scale_pitch": (c_sz, [c_i]),
+    "ag_quantize_e4m3_f32": (c_i, [c_p, c_p, c_i, c_i, c_i] + [c_p] * 4),
+    "ag_matmul_e4m3_f32_workspace": (c_sz, [c_i] * 3),
+    "ag_matmul_e4m3_f32": (c_i, [c_p, c_i, c_i, c_i] + [c_p] * 5 + [c_i, c_p, c_sz]),
+    "ag_quantize_matmul_e4m3_f32_workspace": (c_sz, [c_i] * 3),
+    "ag_quantize_matmul_e4m3_f32": (c_i, [c_p, c_i, c_i, c_i, c_p, c_i, c_p, c_p, c_p, c_i, c_p, c_sz]),
+    "ag_rms_norm_f32": (c_i, [c_p] * 4 + [c_f] + [c_p] * 5 + [c_i, c_i]),
+    "ag_rms_norm_grad_f32_workspace": (c_sz, [c_i] * 2),
+    "ag_rms_norm_grad_f32": (c_i, [c_p] * 8 + [c_i, c_i, c_p, c_sz]),
+    "ag_global_norm_f32_workspace": (c_sz, [c_i, c_p]),
+    "ag_global_norm_f32": (c_i, [c_p, c_i, c_p, c_p, c_f, c_p, c_p, c_sz]),
+    "ag_clip_by_global_norm_f32": (c_i, [c_p, c_i, c_p, c_p, c_p, c_f, c_p, c_p, c_sz]),
+    "ag_adam_update_multi_clipped_f32": (c_i, [c_p, c_i] + [c_p] * 6 + [c_f] * 4 + [c_p]),
     "ag_matmul_f32_static_scratch_bytes": (c_sz, []),
     "ag_matmul_f32_noalloc": (c_i, [c_p, c_i, c_i, c_i, c_i, c_i, c_p, c_i, c_p, c_i, c_p, c_i]),
 }

@@ -24,15 +24,25 @@ __device__ inline void adam_one(float &p, float g, float &m, float &v, float c1,
     p = p - k.alpha * mh;                // adam.rs:49-50
 }
 
+// The gradient as the update takes it: itself, or times the clipping coefficient (one more rounding, which a gradient
+// clipped in a pass of its own would have had too).
+template <bool CLIP>
+__device__ inline float clipped(float g, float coef)
+{
+    return CLIP ? g * coef : g;
+}
+
 // One 128-bit quad per thread (no loop: the grid covers the array, which measured fastest for a
 // streaming read-modify-write); the two bias-correction factors are computed by one lane per
 // block and shared through LDS.  The last partial quad is handled by the final thread.
 // `block` is the block's index within this parameter's share of the grid.
+template <bool CLIP>
 __device__ inline void adam_block(float *__restrict__ p, const float *__restrict__ g, float *__restrict__ m,
                                   float *__restrict__ v, const float *__restrict__ t, size_t n,
-                                  const AdamCoef &k, int vec, size_t block)
+                                  const AdamCoef &k, int vec, size_t block, const float *__restrict__ clip)
 {
     __shared__ float corr[2];
+    const float cf = CLIP ? clip[1] : 1.0f;
     if (threadIdx.x == 0) {
         const float tv = t[0];
         corr[0] = 1.0f / (1.0f - powf(k.b1, tv));  // adam.rs:40
@@ -49,17 +59,17 @@ __device__ inline void adam_block(float *__restrict__ p, const float *__restrict
             float4 mm = ld_stream(reinterpret_cast<const float4 *>(m) + i);
             float4 vv = ld_stream(reinterpret_cast<const float4 *>(v) + i);
             const float4 gg = ld_stream(reinterpret_cast<const float4 *>(g) + i);
-            adam_one(pp.x, gg.x, mm.x, vv.x, c1, c2, rm, rv, k);
-            adam_one(pp.y, gg.y, mm.y, vv.y, c1, c2, rm, rv, k);
-            adam_one(pp.z, gg.z, mm.z, vv.z, c1, c2, rm, rv, k);
-            adam_one(pp.w, gg.w, mm.w, vv.w, c1, c2, rm, rv, k);
+            adam_one(pp.x, clipped<CLIP>(gg.x, cf), mm.x, vv.x, c1, c2, rm, rv, k);
+            adam_one(pp.y, clipped<CLIP>(gg.y, cf), mm.y, vv.y, c1, c2, rm, rv, k);
+            adam_one(pp.z, clipped<CLIP>(gg.z, cf), mm.z, vv.z, c1, c2, rm, rv, k);
+            adam_one(pp.w, clipped<CLIP>(gg.w, cf), mm.w, vv.w, c1, c2, rm, rv, k);
             st_stream(reinterpret_cast<float4 *>(p) + i, pp);
             st_stream(reinterpret_cast<float4 *>(m) + i, mm);
             st_stream(reinterpret_cast<float4 *>(v) + i, vv);
         } else if (i == n4) {
             for (size_t e = n4 * 4; e < n; ++e) {
                 float pp = p[e], mm = m[e], vv = v[e];
-                adam_one(pp, g[e], mm, vv, c1, c2, rm, rv, k);
+                adam_one(pp, clipped<CLIP>(g[e], cf), mm, vv, c1, c2, rm, rv, k);
                 p[e] = pp;
                 m[e] = mm;
                 v[e] = vv;
@@ -67,7 +77,7 @@ __device__ inline void adam_block(float *__restrict__ p, const float *__restrict
         }
     } else if (i < n) {
         float pp = p[i], mm = m[i], vv = v[i];
-        adam_one(pp, g[i], mm, vv, c1, c2, rm, rv, k);
+        adam_one(pp, clipped<CLIP>(g[i], cf), mm, vv, c1, c2, rm, rv, k);
         p[i] = pp;
         m[i] = mm;
         v[i] = vv;
@@ -89,10 +99,13 @@ constexpr size_t kAdamRunFrom = (size_t)1 << 20;  // elements from which the run
 
 // `block` < adam_full_runs(n): every chunk of the run lies inside the array (no bounds tests: with them the
 // compiler waits for every outstanding load and store at each step).
+template <bool CLIP>
 __device__ inline void adam_block_run(float *__restrict__ p, const float *__restrict__ g, float *__restrict__ m,
-                                      float *__restrict__ v, const float *__restrict__ t, const AdamCoef &k, size_t block)
+                                      float *__restrict__ v, const float *__restrict__ t, const AdamCoef &k, size_t block,
+                                      const float *__restrict__ clip)
 {
     __shared__ float corr[2];
+    const float cf = CLIP ? clip[1] : 1.0f;
     if (threadIdx.x == 0) {
         const float tv = t[0];
         corr[0] = 1.0f / (1.0f - powf(k.b1, tv));  // adam.rs:40
@@ -116,10 +129,10 @@ __device__ inline void adam_block_run(float *__restrict__ p, const float *__rest
         if (s >= 3 && s - 3 < kAdamRun) P[s - 3] = ld_stream(p4 + (s - 3) * 256);
         if (s >= 4 && s - 4 < kAdamRun) {
             const int c = s - 4;
-            adam_one(P[c].x, G[c].x, M[c].x, V[c].x, c1, c2, rm, rv, k);
-            adam_one(P[c].y, G[c].y, M[c].y, V[c].y, c1, c2, rm, rv, k);
-            adam_one(P[c].z, G[c].z, M[c].z, V[c].z, c1, c2, rm, rv, k);
-            adam_one(P[c].w, G[c].w, M[c].w, V[c].w, c1, c2, rm, rv, k);
+            adam_one(P[c].x, clipped<CLIP>(G[c].x, cf), M[c].x, V[c].x, c1, c2, rm, rv, k);
+            adam_one(P[c].y, clipped<CLIP>(G[c].y, cf), M[c].y, V[c].y, c1, c2, rm, rv, k);
+            adam_one(P[c].z, clipped<CLIP>(G[c].z, cf), M[c].z, V[c].z, c1, c2, rm, rv, k);
+            adam_one(P[c].w, clipped<CLIP>(G[c].w, cf), M[c].w, V[c].w, c1, c2, rm, rv, k);
             st_stream(p4 + c * 256, P[c]);
         }
         if (s >= 5 && s - 5 < kAdamRun) st_stream(m4 + (s - 5) * 256, M[s - 5]);
@@ -138,20 +151,21 @@ inline size_t adam_blocks(size_t n, int vec)
     const size_t full = adam_full_runs(n), rest = n - full * (size_t)(kAdamRun * 1024);
     return full + (rest / 4 + 1 + 255) / 256;
 }
+template <bool CLIP>
 __device__ inline void adam_entry(float *__restrict__ p, const float *__restrict__ g, float *__restrict__ m,
                                   float *__restrict__ v, const float *__restrict__ t, size_t n, const AdamCoef &k, int vec,
-                                  size_t block)
+                                  size_t block, const float *__restrict__ clip)
 {
     if (vec == 2) {
         const size_t full = adam_full_runs(n);
         if (block < full) {
-            adam_block_run(p, g, m, v, t, k, block);
+            adam_block_run<CLIP>(p, g, m, v, t, k, block, clip);
         } else {
             const size_t off = full * (size_t)(kAdamRun * 1024);
-            adam_block(p + off, g + off, m + off, v + off, t, n - off, k, 1, block - full);
+            adam_block<CLIP>(p + off, g + off, m + off, v + off, t, n - off, k, 1, block - full, clip);
         }
     } else {
-        adam_block(p, g, m, v, t, n, k, vec, block);
+        adam_block<CLIP>(p, g, m, v, t, n, k, vec, block, clip);
     }
 }
 
@@ -160,7 +174,7 @@ __global__ __launch_bounds__(256) void adam_kernel(float *__restrict__ p, const 
                                                    const float *__restrict__ t, size_t n, AdamCoef k,
                                                    int vec)
 {
-    adam_entry(p, g, m, v, t, n, k, vec, blockIdx.x);
+    adam_entry<false>(p, g, m, v, t, n, k, vec, blockIdx.x, nullptr);
 }
 
 // Several parameters in one launch: the table travels in the kernel arguments, each parameter owns
@@ -179,11 +193,12 @@ struct AdamTable {
     int count;
 };
 
-__global__ __launch_bounds__(256) void adam_multi_kernel(AdamTable tab, AdamCoef k)
+template <bool CLIP>
+__global__ __launch_bounds__(256) void adam_multi_kernel(AdamTable tab, AdamCoef k, const float *__restrict__ clip)
 {
     int i = 0;
     while (i + 1 < tab.count && blockIdx.x >= tab.first_block[i + 1]) ++i;
-    adam_entry(tab.p[i], tab.g[i], tab.m[i], tab.v[i], tab.t[i], (size_t)tab.n[i], k, tab.vec[i], blockIdx.x - tab.first_block[i]);
+    adam_entry<CLIP>(tab.p[i], tab.g[i], tab.m[i], tab.v[i], tab.t[i], (size_t)tab.n[i], k, tab.vec[i], blockIdx.x - tab.first_block[i], clip);
 }
 
 // t += 1 for every parameter of the table, after the update kernel has read them (same stream => ordered)
@@ -221,10 +236,10 @@ extern "C" ag_status_t ag_adam_update_f32(ag_stream_t stream, float *param, cons
 
 extern "C" int ag_adam_update_multi_max(void) { return kAdamMultiMax; }
 
-extern "C" ag_status_t ag_adam_update_multi_f32(ag_stream_t stream, int count, float *const *params,
-                                                const float *const *grads, float *const *ms, float *const *vs,
-                                                float *const *ts, const size_t *ns, float alpha, float eps,
-                                                float b1, float b2)
+// `clip` null: the gradients as they are; else times clip[1] (what ag_global_norm_f32 writes).
+static ag_status_t adam_update_multi(ag_stream_t stream, int count, float *const *params, const float *const *grads,
+                                     float *const *ms, float *const *vs, float *const *ts, const size_t *ns, float alpha,
+                                     float eps, float b1, float b2, const float *clip)
 {
     AG_REQUIRE(count >= 0 && count <= kAdamMultiMax, AG_ERR_INVALID_DIMS, "adam: %d parameters in one call (at most %d)",
                count, kAdamMultiMax);
@@ -261,8 +276,27 @@ extern "C" ag_status_t ag_adam_update_multi_f32(ag_stream_t stream, int count, f
     }
     tab.first_block[count] = (unsigned)total;
     hipStream_t st = as_stream(stream);
-    if (total > 0)
-        hipLaunchKernelGGL(adam_multi_kernel, dim3((unsigned)total), dim3(256), 0, st, tab, AdamCoef{alpha, eps, b1, b2});
+    if (total > 0 && clip)
+        hipLaunchKernelGGL(adam_multi_kernel<true>, dim3((unsigned)total), dim3(256), 0, st, tab, AdamCoef{alpha, eps, b1, b2}, clip);
+    else if (total > 0)
+        hipLaunchKernelGGL(adam_multi_kernel<false>, dim3((unsigned)total), dim3(256), 0, st, tab, AdamCoef{alpha, eps, b1, b2}, clip);
     hipLaunchKernelGGL(adam_tick_multi_kernel, dim3(1), dim3(64), 0, st, tab);
     return check_launch("adam");
+}
+
+extern "C" ag_status_t ag_adam_update_multi_f32(ag_stream_t stream, int count, float *const *params,
+                                                const float *const *grads, float *const *ms, float *const *vs,
+                                                float *const *ts, const size_t *ns, float alpha, float eps,
+                                                float b1, float b2)
+{
+    return adam_update_multi(stream, count, params, grads, ms, vs, ts, ns, alpha, eps, b1, b2, nullptr);
+}
+
+extern "C" ag_status_t ag_adam_update_multi_clipped_f32(ag_stream_t stream, int count, float *const *params,
+                                                        const float *const *grads, float *const *ms, float *const *vs,
+                                                        float *const *ts, const size_t *ns, float alpha, float eps,
+                                                        float b1, float b2, const float *clip)
+{
+    AG_REQUIRE(clip, AG_ERR_INVALID_DIMS, "adam: null clipping coefficient");
+    return adam_update_multi(stream, count, params, grads, ms, vs, ts, ns, alpha, eps, b1, b2, clip);
 }

@@ -5,7 +5,8 @@
 set -euo pipefail
 here="$(cd "$(dirname "${BASH_SOURCE[0]}")" && pwd)"
 out="$here/../libag_hip.so"
-srcs=(common.hip im2col.hip gemm.hip gemm_dl.hip conv.hip conv_s2.hip pool.hip reduce.hip adam.hip elementwise.hip)
+srcs=(common.hip im2col.hip gemm.hip gemm_dl.hip conv.hip conv_s2.hip pool.hip reduce.hip adam.hip elementwise.hip
+      quantize.hip gemm_e4m3.hip norm.hip clip.hip)
 hooked=(gemm.hip pool.hip)   # the sources that hold test hooks: compiled a second time for the test flavour
 flags=(--offload-arch=gfx950 -O3 -std=c++17 -fPIC -fvisibility=hidden
        -Xclang -target-feature -Xclang -packed-fp32-ops
@@ -18,7 +19,7 @@ compile() {  # source, object, extra flags...
   # adam.hip must keep the reference's separately rounded multiplies and adds
   [ "$s" = adam.hip ] && extra+=(-ffp-contract=off)
   # keep the MFMA accumulators in ordinary VGPRs (no copies to and from AGPRs around the epilogue)
-  [ "$s" = gemm_dl.hip ] && extra+=(-Wno-inline-asm -Wno-pass-failed)
+  { [ "$s" = gemm_dl.hip ] || [ "$s" = gemm_e4m3.hip ]; } && extra+=(-Wno-inline-asm -Wno-pass-failed)
   /opt/rocm/bin/hipcc "${flags[@]}" "${extra[@]}" -c "$here/$s" -o "$o" &
   pids+=($!)
 }

@@ -1,0 +1,436 @@
+// Matrix product of two e4m3 operands whose scales stand beside them: C[M,N] = A[M,K] . B[N,K]^T in f32, both operands
+// contiguous along the contraction.
+//
+// Operands stay in 8 bits in HBM and LDS and become bf16 on the way into the matrix unit: one instruction
+// (v_cvt_scalef32_pk_bf16_fp8) turns two values into bf16 and multiplies them by the block's power of two, all of it
+// exact (4 significant bits, an exponent that bf16 holds).  The 8-bit matrix instruction v_mfma_scale_f32_32x32x64_f8f6f4
+// would multiply twice as fast, but it does not keep f32 sums: it aligns each group of 8 products to the largest of them
+// and drops what lies 2^-14 below (measured: +2^16 - 2^16 + 2^2 within a group gives 0), 1.4e-5 of the result for
+// Gaussian operands and 6e-5 for wider ones, whatever the length; the bf16 instruction gives 8e-8 and 4e-7.
+#include "e4m3.h"
+
+namespace ag {
+
+typedef int v2i __attribute__((ext_vector_type(2)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+struct GemmE4m3 {
+    const unsigned char *a, *a_scales, *b, *b_scales;
+    float *c;
+    long long ldc, pitch;
+    int M, N, blocks, scale_pitch;  // blocks of 128 along the contraction
+    int tiles_m, tiles_n;
+    int splits, per_split;  // slices of the contraction and blocks of 128 in each; splits > 1: c is [splits][M][N]
+};
+
+// The factor that a scale byte stands for (bytes 1..254; 0 stands for 2^-127, which no block that this library rounds has).
+__device__ inline float scale_factor(unsigned word, int i) { return __uint_as_float(((word >> (8 * i)) & 0xffu) << 23); }
+
+// Eight consecutive e4m3 values times s, in bf16.
+__device__ inline v8bf widen(int lo, int hi, float s)
+{
+    const v2bf r0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false), r1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true);
+    const v2bf r2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false), r3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true);
+    return v8bf{r0[0], r0[1], r1[0], r1[1], r2[0], r2[1], r3[0], r3[1]};
+}
+
+// ---- tiles ------------------------------------------------------------------------------------------------------------
+typedef __attribute__((address_space(3))) unsigned char lds_byte_t;
+
+// Loads straight from global memory into LDS: lane l's 16 (or 4) bytes land at lds + 16 l (4 l).  In assembly because the
+// compiler would wait for every outstanding load in front of each LDS read; the waits are written out below.
+__device__ inline void dma16(const unsigned char *base, unsigned offset, unsigned lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "m0", "memory");
+}
+__device__ inline void dma4(const unsigned char *base, unsigned offset, unsigned lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "m0", "memory");
+}
+__device__ inline const unsigned char *uniform(const unsigned char *p)
+{
+    const unsigned long long b = reinterpret_cast<unsigned long long>(p);
+    const unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)b), hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(b >> 32));
+    return reinterpret_cast<const unsigned char *>(((unsigned long long)hi << 32) | lo);
+}
+
+// BM x BN of C per block, WM x WN per wave, 128 of the contraction per step.  LDS holds two steps of both operands, rows of
+// 128 bytes; the 16-byte piece c of row r stands at place c ^ (r & 7), so that the 32 rows that a half wave reads at one
+// piece fall on all banks.  A step's loads are issued at the start of the step before it, behind the barrier that ends
+// the reads of that buffer; its scales come four steps at a time (one word per row), in a second pair of buffers.
+template <int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void gemm_e4m3_tile_kernel(GemmE4m3 p)
+{
+    constexpr int WAVES_N = BN / WN, NW = BM / WM * WAVES_N, MI = WM / 32, NI = WN / 32;
+    constexpr int ROWS = BM + BN, STEP = ROWS * 128;
+    constexpr int LOADS = ROWS / 8 / NW;  // 1 KiB loads (8 rows) of a wave per step
+    constexpr int SCALE_LOADS = ROWS / 64;
+    static_assert(ROWS % (8 * NW) == 0 && BM % 64 == 0 && BN % 64 == 0 && SCALE_LOADS <= NW, "rows divide over the waves");
+    __shared__ __attribute__((aligned(1024))) unsigned char tile[2 * STEP];
+    __shared__ __attribute__((aligned(256))) unsigned scale_words[2][ROWS];
+    const unsigned lds = (unsigned)(size_t)(lds_byte_t *)tile, lds_scales = (unsigned)(size_t)(lds_byte_t *)scale_words;
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WAVES_N, wn = wave % WAVES_N;
+
+    // Consecutive places go down bands of 8 tile rows: the 32 blocks that an XCD runs at a time form a patch of 8 x 4 tiles.
+    const unsigned total = (unsigned)p.tiles_m * p.tiles_n;
+    unsigned place = xcd_remap(blockIdx.x, gridDim.x);
+    const int split = (int)(place / total);
+    place -= (unsigned)split * total;
+    const unsigned band = place / (8u * p.tiles_n), rest = place - band * 8u * p.tiles_n;
+    const unsigned high = min(8u, (unsigned)p.tiles_m - band * 8u);
+    const int m0 = (int)(band * 8u + rest % high) * BM, n0 = (int)(rest / high) * BN;
+
+    // what this lane fetches: rows of 128 bytes, 8 lanes each
+    const unsigned char *base[LOADS];
+    unsigned offset[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int r0 = (i * NW + wave) * 8;  // (a group of 8 rows lies in one operand)
+        const bool in_a = r0 < BM;
+        const int first = in_a ? m0 + r0 : n0 + r0 - BM, last = (in_a ? p.M : p.N) - 1;
+        const int start = min(first, last), row = min(first + (lane >> 3), last);
+        base[i] = uniform((in_a ? p.a : p.b) + start * p.pitch);
+        // (a row's pitch is at most 2^31: 8 rows pass 32 bits only where one row is longer than 2^28, which the host refuses)
+        offset[i] = (unsigned)((row - start) * p.pitch) + (unsigned)(((lane & 7) ^ (lane >> 3)) * 16);
+    }
+    const unsigned char *scale_base = nullptr;
+    unsigned scale_offset = 0;
+    if (wave < SCALE_LOADS) {
+        const int r0 = wave * 64;
+        const bool in_a = r0 < BM;
+        const int first = in_a ? m0 + r0 : n0 + r0 - BM, last = (in_a ? p.M : p.N) - 1;
+        const int start = min(first, last), row = min(first + lane, last);
+        scale_base = uniform((in_a ? p.a_scales : p.b_scales) + (long long)start * p.scale_pitch);
+        scale_offset = (unsigned)((row - start) * p.scale_pitch);
+    }
+
+    const int k_begin = split * p.per_split, k_end = min(p.blocks, k_begin + p.per_split);
+    auto fetch = [&](int k, int buffer) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            dma16(base[i] + (long long)k * 128, offset[i], lds + (unsigned)(buffer * STEP + (i * NW + wave) * 1024));
+        if ((k & 3) == 0 || k == k_begin) {  // (a slice may begin inside a word)
+            if (wave < SCALE_LOADS) dma4(scale_base + (k & ~3), scale_offset, lds_scales + (unsigned)(((k >> 2) & 1) * ROWS * 4 + wave * 256));
+        }
+    };
+
+    v16f acc[MI][NI] = {};
+    const int row_a = wm * WM + (lane & 31), row_b = BM + wn * WN + (lane & 31);
+    if (k_begin < k_end) fetch(k_begin, 0);
+    unsigned word_a[MI], word_b[NI];
+    for (int k = k_begin, buffer = 0; k < k_end; ++k, buffer ^= 1) {
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" : : : "memory");
+        if (k + 1 < k_end) fetch(k + 1, buffer ^ 1);
+        if ((k & 3) == 0 || k == k_begin) {
+#pragma unroll
+            for (int i = 0; i < MI; ++i) word_a[i] = scale_words[(k >> 2) & 1][row_a + i * 32];
+#pragma unroll
+            for (int j = 0; j < NI; ++j) word_b[j] = scale_words[(k >> 2) & 1][row_b + j * 32];
+        }
+        float sa[MI], sb[NI];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) sa[i] = scale_factor(word_a[i], k & 3);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) sb[j] = scale_factor(word_b[j], k & 3);
+        const unsigned char *at = tile + buffer * STEP;
+#pragma unroll
+        for (int c = 0; c < 8; c += 2) {  // 32 of the contraction: the half waves take a 16-byte piece each
+            const int piece = ((c + (lane >> 5)) ^ (lane & 7)) * 16;
+            v4i qa[MI], qb[NI];
+#pragma unroll
+            for (int i = 0; i < MI; ++i) qa[i] = *reinterpret_cast<const v4i *>(at + (row_a + i * 32) * 128 + piece);
+#pragma unroll
+            for (int j = 0; j < NI; ++j) qb[j] = *reinterpret_cast<const v4i *>(at + (row_b + j * 32) * 128 + piece);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                v8bf va[MI], vb[NI];
+#pragma unroll
+                for (int i = 0; i < MI; ++i) va[i] = widen(qa[i][2 * h], qa[i][2 * h + 1], sa[i]);
+#pragma unroll
+                for (int j = 0; j < NI; ++j) vb[j] = widen(qb[j][2 * h], qb[j][2 * h + 1], sb[j]);
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[i], vb[j], acc[i][j], 0, 0, 0);
+            }
+        }
+    }
+    float *c = p.c + (long long)split * p.M * p.ldc;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+            const int n = n0 + wn * WN + j * 32 + (lane & 31);
+            const int m = m0 + wm * WM + i * 32 + 4 * (lane >> 5);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int r = m + 8 * (e / 4) + e % 4;
+                if (r < p.M && n < p.N) c[r * p.ldc + n] = acc[i][j][e];
+            }
+        }
+}
+
+// C = the slices' partial results added in order.
+__global__ __launch_bounds__(256) void gemm_e4m3_fold_kernel(const float *__restrict__ partial, float *__restrict__ c, long long ldc, int M, int N, int splits)
+{
+    const long long i = (long long)blockIdx.x * 1024 + threadIdx.x * 4, cells = (long long)M * N;
+    if (i >= cells) return;
+    quad_t s = load_quad(partial, i, cells);
+    for (int k = 1; k < splits; ++k) s += load_quad(partial + k * cells, i, cells);
+    const long long m = i / N, n = i - m * N;
+    if (n + 4 <= N) {
+        *reinterpret_cast<quad_any_t *>(c + m * ldc + n) = s;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const long long at = i + j;
+            if (at < cells) c[at / N * ldc + at % N] = s[j];
+        }
+    }
+}
+
+// ---- few rows ---------------------------------------------------------------------------------------------------------
+// Up to 16 * MT rows of A against 16 rows of B per block, operands straight from global memory into the matrix unit's
+// layout: the weight is read once, in whole 512-byte pieces of its rows, and nothing is shared between waves but the
+// sums.  The waves take pieces of 512 of the contraction in turn; their sums are added in order through LDS.
+// Lane l holds row l % 16 and 32 consecutive bytes of each 128: group l / 16 of four.
+// FROM_F32: A is x itself, rounded on the way as ag_quantize_e4m3_f32 rounds it.
+constexpr int kSkinnyRows = 64;
+
+template <int MT, int NW, bool FROM_F32>
+__global__ __launch_bounds__(NW * 64) void gemm_e4m3_skinny_kernel(GemmE4m3 p, const float *__restrict__ x, long long ldx, int K)
+{
+    static_assert(!FROM_F32 || MT == 1, "rounded in place for few rows only");
+    __shared__ float sums[NW][MT][256];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r16 = lane & 15, group = lane >> 4;
+    const int n0 = blockIdx.x * 16;
+    const int row_b = min(n0 + r16, p.N - 1);
+    const unsigned char *b = p.b + row_b * p.pitch + group * 32, *b_scales = p.b_scales + (long long)row_b * p.scale_pitch;
+    const int words = (p.blocks + 3) / 4;
+    v4f acc[MT] = {};
+    for (int w = wave; w < words; w += NW) {
+        const int count = min(4, p.blocks - w * 4);
+        v4i qb[4][2];
+        const unsigned word_b = *reinterpret_cast<const unsigned *>(b_scales + w * 4);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (u < count)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) qb[u][h] = *reinterpret_cast<const v4i *>(b + (long long)(w * 4 + u) * 128 + h * 16);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            v4i qa[4][2];
+            unsigned word_a = 0;
+            if (FROM_F32) {
+                const bool here = r16 < p.M;
+                const float *row = x + (here ? r16 : 0) * ldx;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (u < count) {
+                        quad_t v[8];
+                        unsigned top = 0;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            v[i] = here ? load_quad(row, (long long)(w * 4 + u) * 128 + group * 32 + i * 4, K) : quad_t{0.f, 0.f, 0.f, 0.f};
+                            top = max(top, finite_magnitude(v[i]));
+                        }
+                        top = max(top, (unsigned)__shfl_xor((int)top, 16, 64));
+                        top = max(top, (unsigned)__shfl_xor((int)top, 32, 64));
+                        const unsigned sb = scale_byte(top);
+                        const float inv = scale_inverse(sb);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) qa[u][i / 4][i % 4] = (int)round_e4m3(v[i], inv);
+                        word_a |= sb << (8 * u);
+                    }
+            } else {
+                const int row_a = min(t * 16 + r16, p.M - 1);
+                word_a = *reinterpret_cast<const unsigned *>(p.a_scales + (long long)row_a * p.scale_pitch + w * 4);
+                const unsigned char *a = p.a + row_a * p.pitch + group * 32;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (u < count)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) qa[u][h] = *reinterpret_cast<const v4i *>(a + (long long)(w * 4 + u) * 128 + h * 16);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (u < count) {
+                    const float sa = scale_factor(word_a, u), sb = scale_factor(word_b, u);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(qa[u][h][2 * e], qa[u][h][2 * e + 1], sa),
+                                                                            widen(qb[u][h][2 * e], qb[u][h][2 * e + 1], sb), acc[t], 0, 0, 0);
+                }
+        }
+    }
+    // lane l holds column l % 16 and rows 4 (l / 16) .. + 3
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sums[wave][t][(group * 4 + e) * 16 + r16] = acc[t][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < MT * 256; i += NW * 64) {
+        float s = sums[0][i / 256][i % 256];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) s += sums[w][i / 256][i % 256];
+        const int m = i / 16, n = n0 + i % 16;
+        if (m < p.M && n < p.N) p.c[m * p.ldc + n] = s;
+    }
+}
+
+// ---- which form, and its launch ---------------------------------------------------------------------------------------
+// The rounding of ag_quantize_e4m3_f32 (quantize.hip).
+ag_status_t quantize_e4m3(const char *who, hipStream_t st, const float *x, long long ldx, int rows, int cols, unsigned char *q, unsigned char *scales,
+                          unsigned char *qt, unsigned char *scales_t);
+
+struct Plan {
+    int bm, bn, splits;
+};
+
+static Plan plan_product(int M, int N, int K)
+{
+    const long long blocks = (long long)(e4m3_pitch(K) / kE4m3Block), cus = device_cus();
+    auto tiles = [&](int t) { return (long long)((M + t - 1) / t) * ((N + t - 1) / t); };
+    Plan f = {256, 256, 1};
+    if (tiles(256) < cus * 3 / 4) {
+        f = {128, 128, 1};
+        const long long want = (2 * cus) / (tiles(128) ? tiles(128) : 1);
+        f.splits = (int)(want < 1 ? 1 : want > 16 ? 16 : want);
+        while (f.splits > 1 && blocks / f.splits < 4) --f.splits;
+    }
+    return f;
+}
+
+static size_t product_workspace(int M, int N, int K)
+{
+    if (M <= 0 || N <= 0 || K <= 0 || M <= kSkinnyRows) return 0;
+    const Plan f = plan_product(M, N, K);
+    return f.splits > 1 ? (size_t)f.splits * M * N * sizeof(float) : 0;
+}
+
+static ag_status_t check_product(const char *who, int M, int N, int K, int ldc, const void *b, const void *bs, const void *c)
+{
+    AG_REQUIRE(M >= 0 && N >= 0 && K >= 0, AG_ERR_INVALID_DIMS, "%s: negative extent (%d x %d x %d)", who, M, N, K);
+    AG_REQUIRE(K <= 1 << 28, AG_ERR_INVALID_DIMS, "%s: a contraction of %d elements (at most 2^28)", who, K);
+    AG_REQUIRE(ldc >= N, AG_ERR_INCOMPATIBLE_SHAPE, "%s: ldc (%d) is less than a row of %d elements", who, ldc, N);
+    if (M == 0 || N == 0) return AG_OK;
+    AG_REQUIRE(c && (K == 0 || (b && bs)), AG_ERR_INVALID_DIMS, "%s: null pointer", who);
+    AG_REQUIRE(aligned16(b), AG_ERR_INVALID_DIMS, "%s: 8-bit operands must be 16-byte aligned", who);
+    AG_REQUIRE((reinterpret_cast<uintptr_t>(bs) & 3u) == 0, AG_ERR_INVALID_DIMS, "%s: scales must be 4-byte aligned", who);
+    return AG_OK;
+}
+
+template <int MT, bool FROM_F32>
+static void launch_skinny(hipStream_t st, const GemmE4m3 &p, const float *x, long long ldx, int K)
+{
+    const dim3 grid((unsigned)((p.N + 15) / 16));
+    const int words = (p.blocks + 3) / 4;
+    if (words <= 2)
+        hipLaunchKernelGGL((gemm_e4m3_skinny_kernel<MT, 2, FROM_F32>), grid, dim3(128), 0, st, p, x, ldx, K);
+    else if (words <= 4)
+        hipLaunchKernelGGL((gemm_e4m3_skinny_kernel<MT, 4, FROM_F32>), grid, dim3(256), 0, st, p, x, ldx, K);
+    else
+        hipLaunchKernelGGL((gemm_e4m3_skinny_kernel<MT, 8, FROM_F32>), grid, dim3(512), 0, st, p, x, ldx, K);
+}
+
+static ag_status_t product(const char *who, hipStream_t st, GemmE4m3 p, int K, void *ws)
+{
+    if (p.M <= kSkinnyRows) {
+        if (p.M <= 16) launch_skinny<1, false>(st, p, nullptr, 0, K);
+        else if (p.M <= 32) launch_skinny<2, false>(st, p, nullptr, 0, K);
+        else if (p.M <= 48) launch_skinny<3, false>(st, p, nullptr, 0, K);
+        else launch_skinny<4, false>(st, p, nullptr, 0, K);
+        return check_launch(who);
+    }
+    const Plan f = plan_product(p.M, p.N, K);
+    p.tiles_m = (p.M + f.bm - 1) / f.bm;
+    p.tiles_n = (p.N + f.bn - 1) / f.bn;
+    p.splits = f.splits;
+    p.per_split = (p.blocks + f.splits - 1) / f.splits;
+    const unsigned long long grid = (unsigned long long)p.tiles_m * p.tiles_n * f.splits;
+    AG_REQUIRE(grid <= (unsigned long long)kMaxGridX, AG_ERR_INVALID_DIMS, "%s: too many tiles (%llu)", who, grid);
+    float *c = p.c;
+    const long long ldc = p.ldc;
+    if (f.splits > 1) p.c = static_cast<float *>(ws), p.ldc = p.N;
+    if (f.bm == 256)
+        hipLaunchKernelGGL((gemm_e4m3_tile_kernel<256, 256, 128, 64>), dim3((unsigned)grid), dim3(512), 0, st, p);
+    else
+        hipLaunchKernelGGL((gemm_e4m3_tile_kernel<128, 128, 64, 64>), dim3((unsigned)grid), dim3(256), 0, st, p);
+    if (f.splits > 1) {
+        const long long cells = (long long)p.M * p.N;
+        hipLaunchKernelGGL(gemm_e4m3_fold_kernel, dim3((unsigned)((cells + 1023) / 1024)), dim3(256), 0, st, static_cast<const float *>(ws), c, ldc, p.M,
+                           p.N, f.splits);
+    }
+    return check_launch(who);
+}
+
+static GemmE4m3 params(int M, int N, int K, const unsigned char *a, const unsigned char *as, const unsigned char *b, const unsigned char *bs, float *c,
+                       int ldc)
+{
+    GemmE4m3 p = {a, as, b, bs, c, ldc, (long long)e4m3_pitch(K), M, N, (int)(e4m3_pitch(K) / kE4m3Block), (int)e4m3_scale_pitch(K), 0, 0, 1, 0};
+    return p;
+}
+
+// Workspace of the product from f32: the rounded x and its scales, then the product's own.
+static size_t rounded_bytes(int M, int K) { return (size_t)M * e4m3_pitch(K) + ((size_t)M * e4m3_scale_pitch(K) + 15) / 16 * 16; }
+
+// Few enough rows of x that each block rounds them for itself.
+static bool rounds_in_place(int M) { return M <= 4; }
+
+}  // namespace ag
+
+using namespace ag;
+
+extern "C" size_t ag_matmul_e4m3_f32_workspace(int M, int N, int K) { return product_workspace(M, N, K); }
+
+extern "C" ag_status_t ag_matmul_e4m3_f32(ag_stream_t stream, int M, int N, int K, const uint8_t *A, const uint8_t *a_scales, const uint8_t *B,
+                                          const uint8_t *b_scales, float *C, int ldc, void *ws, size_t ws_bytes)
+{
+    const ag_status_t e = check_product("matmul_e4m3", M, N, K, ldc, B, b_scales, C);
+    if (e != AG_OK) return e;
+    if (M == 0 || N == 0) return AG_OK;
+    AG_REQUIRE(K == 0 || (A && a_scales), AG_ERR_INVALID_DIMS, "matmul_e4m3: null pointer");
+    AG_REQUIRE(aligned16(A), AG_ERR_INVALID_DIMS, "matmul_e4m3: 8-bit operands must be 16-byte aligned");
+    AG_REQUIRE((reinterpret_cast<uintptr_t>(a_scales) & 3u) == 0, AG_ERR_INVALID_DIMS, "matmul_e4m3: scales must be 4-byte aligned");
+    const size_t need = product_workspace(M, N, K);
+    AG_REQUIRE(need == 0 || (ws && ws_bytes >= need), AG_ERR_INVALID_DIMS, "matmul_e4m3: workspace of %zu bytes, %zu needed", ws_bytes, need);
+    AG_REQUIRE(need == 0 || aligned16(ws), AG_ERR_INVALID_DIMS, "matmul_e4m3: misaligned workspace");
+    return product("matmul_e4m3", as_stream(stream), params(M, N, K, A, a_scales, B, b_scales, C, ldc), K, ws);
+}
+
+extern "C" size_t ag_quantize_matmul_e4m3_f32_workspace(int M, int N, int K)
+{
+    if (M <= 0 || N <= 0 || K <= 0 || rounds_in_place(M)) return 0;
+    return rounded_bytes(M, K) + product_workspace(M, N, K);
+}
+
+extern "C" ag_status_t ag_quantize_matmul_e4m3_f32(ag_stream_t stream, int M, int N, int K, const float *x, int ldx, const uint8_t *B,
+                                                   const uint8_t *b_scales, float *C, int ldc, void *ws, size_t ws_bytes)
+{
+    ag_status_t e = check_product("quantize_matmul_e4m3", M, N, K, ldc, B, b_scales, C);
+    if (e != AG_OK) return e;
+    AG_REQUIRE(ldx >= K, AG_ERR_INCOMPATIBLE_SHAPE, "quantize_matmul_e4m3: ldx (%d) is less than a row of %d elements", ldx, K);
+    if (M == 0 || N == 0) return AG_OK;
+    AG_REQUIRE(K == 0 || x, AG_ERR_INVALID_DIMS, "quantize_matmul_e4m3: null pointer");
+    const size_t need = ag_quantize_matmul_e4m3_f32_workspace(M, N, K);
+    AG_REQUIRE(need == 0 || (ws && ws_bytes >= need), AG_ERR_INVALID_DIMS, "quantize_matmul_e4m3: workspace of %zu bytes, %zu needed", ws_bytes, need);
+    AG_REQUIRE(need == 0 || aligned16(ws), AG_ERR_INVALID_DIMS, "quantize_matmul_e4m3: misaligned workspace");
+    hipStream_t st = as_stream(stream);
+    if (rounds_in_place(M)) {
+        launch_skinny<1, true>(st, params(M, N, K, nullptr, nullptr, B, b_scales, C, ldc), x, ldx, K);
+        return check_launch("quantize_matmul_e4m3");
+    }
+    unsigned char *q = static_cast<unsigned char *>(ws), *scales = q + (size_t)M * e4m3_pitch(K);
+    e = quantize_e4m3("quantize_matmul_e4m3", st, x, ldx, M, K, q, scales, nullptr, nullptr);
+    if (e != AG_OK) return e;
+    return product("quantize_matmul_e4m3", st, params(M, N, K, q, scales, B, b_scales, C, ldc), K, q + rounded_bytes(M, K));
+}

@@ -1,0 +1,342 @@
+// Root-mean-square norm of a row, with the addition of a residual in front of it and the rounding to e4m3 behind it in
+// the same pass, and its gradient.
+//
+//   h = x + residual           y = h * r * w,   r = 1 / sqrt(mean(h^2) + eps)
+//   gx = r (w gy) - h r^3 / n * sum(w gy h) (+ gh)          gw = sum over rows of gy h r
+//
+// The sum of squares, r and the two products of y are in 64 bits and y is rounded to f32 once, so that the same row gives
+// the same f32 value however the sum is ordered, and the rounding to 8 bits behind it -- where neighbouring values are 6 %
+// apart -- does not depend on the launch shape.  The passes are bound by HBM; 64-bit arithmetic is free there.
+#include "e4m3.h"
+
+namespace ag {
+
+// Sum over the block, the same value in every thread.  `part`: one double per wave.
+template <int T>
+__device__ inline double block_sum(double v, double *part)
+{
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
+    if (T == 64) return v;
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < T / 64; ++i) s += part[i];
+    return s;
+}
+
+struct NormArgs {
+    const float *x, *residual, *weight;
+    float *h, *y, *rstd;
+    unsigned char *q, *scales;
+    double eps;
+    long long n;
+    unsigned nb, nbp;
+};
+
+__device__ inline quad_t norm_quad(quad_t h, quad_t w, double r)
+{
+    quad_t y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = (float)((double)h[j] * r * (double)w[j]);
+    return y;
+}
+__device__ inline double square_sum(quad_t h, double s)
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s = fma((double)h[j], (double)h[j], s);
+    return s;
+}
+
+// Writes what the quad at element i of a row gives: the f32 value, and its share of the 8-bit block, which the 32 lanes
+// of the half wave hold between them (all of them call this together: the maximum runs over the half wave).
+__device__ inline void norm_write(const NormArgs &a, size_t row, long long i, quad_t y)
+{
+    if (a.y && i < a.n) store_quad(a.y + row * a.n, i, a.n, y);
+    if (a.q) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i + j >= a.n) y[j] = 0.f;  // (padding stays zero where r is not finite)
+        const unsigned sb = scale_byte(half_wave_max(finite_magnitude(y)));
+        const long long b = i / kE4m3Block;
+        if (b < a.nb) *reinterpret_cast<unsigned *>(a.q + (row * a.nb) * kE4m3Block + i) = round_e4m3(y, scale_inverse(sb));
+        if ((threadIdx.x & 31) == 0 && b < a.nbp) a.scales[row * a.nbp + b] = (unsigned char)sb;
+    }
+}
+
+// One row per T threads, held in registers (Q quads a thread: rows of up to 4 * Q * T elements), so every input is read
+// once; T = 64 packs four rows into a block of 256.  Behind the row's end quads are zero: they pad the 8-bit output.
+template <int T, int Q>
+__global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_kernel(NormArgs a, unsigned rows)
+{
+    __shared__ double part[T / 64];
+    const unsigned t = T == 64 ? threadIdx.x & 63u : threadIdx.x;
+    const size_t row = T == 64 ? (size_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    if (row >= rows) return;  // (whole waves, and only where T == 64, which has no barrier)
+    const float *x = a.x + row * a.n;
+    const float *res = a.residual ? a.residual + row * a.n : nullptr;
+    quad_t h[Q], w[Q];
+#pragma unroll
+    for (int k = 0; k < Q; ++k) h[k] = load_quad(x, (long long)(k * T + t) * 4, a.n);
+    if (res) {
+        quad_t b[Q];
+#pragma unroll
+        for (int k = 0; k < Q; ++k) b[k] = load_quad(res, (long long)(k * T + t) * 4, a.n);
+#pragma unroll
+        for (int k = 0; k < Q; ++k) h[k] += b[k];
+    }
+#pragma unroll
+    for (int k = 0; k < Q; ++k) w[k] = load_quad(a.weight, (long long)(k * T + t) * 4, a.n);
+    double s = 0.0;
+#pragma unroll
+    for (int k = 0; k < Q; ++k) s = square_sum(h[k], s);
+    s = block_sum<T>(s, part);  // (its barrier also orders every read of the row before the writes: outputs may be the inputs)
+    const double r = 1.0 / sqrt(s / (double)a.n + a.eps);
+    if (a.rstd && t == 0) a.rstd[row] = (float)r;
+#pragma unroll
+    for (int k = 0; k < Q; ++k) {
+        const long long i = (long long)(k * T + t) * 4;
+        if (a.h && i < a.n) store_quad(a.h + row * a.n, i, a.n, h[k]);
+        norm_write(a, row, i, norm_quad(h[k], w[k], r));
+    }
+}
+
+// Rows beyond what the registers hold: two passes over the row, the second from cache where it fits.  A thread reads in
+// the second pass only what it read (or wrote, as h) in the first, so outputs may be the inputs here too.
+constexpr int kLongT = 1024;
+__global__ __launch_bounds__(kLongT) void rms_norm_long_kernel(NormArgs a)
+{
+    __shared__ double part[kLongT / 64];
+    const size_t row = blockIdx.x;
+    const float *x = a.x + row * a.n;
+    const float *res = a.residual ? a.residual + row * a.n : nullptr;
+    const long long end = (a.n + kE4m3Block * 4 - 1) / (kE4m3Block * 4) * (kE4m3Block * 4);  // whole groups of four blocks: the scales' padding too
+    double s = 0.0;
+    for (long long i = (long long)threadIdx.x * 4; i < a.n; i += kLongT * 4) {
+        quad_t h = load_quad(x, i, a.n);
+        if (res) h += load_quad(res, i, a.n);
+        s = square_sum(h, s);
+        if (a.h) store_quad(a.h + row * a.n, i, a.n, h);
+    }
+    s = block_sum<kLongT>(s, part);
+    const double r = 1.0 / sqrt(s / (double)a.n + a.eps);
+    if (a.rstd && threadIdx.x == 0) a.rstd[row] = (float)r;
+    for (long long i = (long long)threadIdx.x * 4; i < end; i += kLongT * 4) {
+        quad_t h = load_quad(a.h ? a.h + row * a.n : x, i, a.n);
+        if (!a.h && res) h += load_quad(res, i, a.n);
+        norm_write(a, row, i, norm_quad(h, load_quad(a.weight, i, a.n), r));
+    }
+}
+
+// ---- gradient ---------------------------------------------------------------------------------------------------------
+struct NormGradArgs {
+    const float *h, *weight, *rstd, *gy, *gh;
+    float *gx, *partial;  // partial: [gridDim.x][n] sums of gw, or null
+    long long n;
+};
+
+__device__ inline double dot3(quad_t g, quad_t w, quad_t h, double s)
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s = fma((double)g[j] * (double)w[j], (double)h[j], s);
+    return s;
+}
+__device__ inline quad_t grad_quad(quad_t h, quad_t w, quad_t g, float r, float c)
+{
+    quad_t o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = fmaf(-h[j], c, g[j] * w[j] * r);
+    return o;
+}
+
+// A block walks the rows b, b + G, ... with the row in registers and its share of gw beside it: gw costs one [G][n]
+// array of partial sums, folded in a fixed order below, instead of a second pass over gy and h.
+template <int T, int Q>
+__global__ __launch_bounds__(T) void rms_norm_grad_kernel(NormGradArgs a, unsigned rows)
+{
+    __shared__ double part[2][T / 64];
+    const unsigned t = threadIdx.x;
+    quad_t w[Q], acc[Q];
+#pragma unroll
+    for (int k = 0; k < Q; ++k) {
+        w[k] = load_quad(a.weight, (long long)(k * T + t) * 4, a.n);
+        acc[k] = quad_t{0.f, 0.f, 0.f, 0.f};
+    }
+    int turn = 0;
+    for (size_t row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
+        const float *hr = a.h + row * a.n, *gr = a.gy + row * a.n;
+        quad_t h[Q], g[Q];
+#pragma unroll
+        for (int k = 0; k < Q; ++k) {
+            h[k] = load_quad(hr, (long long)(k * T + t) * 4, a.n);
+            g[k] = load_quad(gr, (long long)(k * T + t) * 4, a.n);
+        }
+        const float r = a.rstd[row];
+        double s = 0.0;
+#pragma unroll
+        for (int k = 0; k < Q; ++k) s = dot3(g[k], w[k], h[k], s);
+        s = block_sum<T>(s, part[turn]);  // (two arrays in turn: the next row's sums do not wait for this row's readers)
+        const float c = (float)(s / (double)a.n * (double)r * (double)r * (double)r);
+#pragma unroll
+        for (int k = 0; k < Q; ++k) {
+            const long long i = (long long)(k * T + t) * 4;
+            if (a.gx && i < a.n) {
+                quad_t o = grad_quad(h[k], w[k], g[k], r, c);
+                if (a.gh) o += load_quad(a.gh + row * a.n, i, a.n);
+                store_quad(a.gx + row * a.n, i, a.n, o);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[k][j] = fmaf(g[k][j], h[k][j] * r, acc[k][j]);
+        }
+    }
+    if (a.partial) {
+        float *p = a.partial + (size_t)blockIdx.x * a.n;
+#pragma unroll
+        for (int k = 0; k < Q; ++k) {
+            const long long i = (long long)(k * T + t) * 4;
+            if (i < a.n) store_quad(p, i, a.n, acc[k]);
+        }
+    }
+}
+
+// Rows beyond the registers: the weight's sums first (gx may be gy or gh), then gx in two passes over each row.
+__global__ __launch_bounds__(256) void rms_norm_grad_weight_long_kernel(NormGradArgs a, unsigned rows)
+{
+    const long long i = ((long long)blockIdx.y * 256 + threadIdx.x) * 4;
+    if (i >= a.n) return;
+    quad_t acc = {0.f, 0.f, 0.f, 0.f};
+    for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const quad_t h = load_quad(a.h + row * a.n, i, a.n), g = load_quad(a.gy + row * a.n, i, a.n);
+        const float r = a.rstd[row];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = fmaf(g[j], h[j] * r, acc[j]);
+    }
+    store_quad(a.partial + (size_t)blockIdx.x * a.n, i, a.n, acc);
+}
+__global__ __launch_bounds__(kLongT) void rms_norm_grad_long_kernel(NormGradArgs a)
+{
+    __shared__ double part[kLongT / 64];
+    const size_t row = blockIdx.x;
+    const float *hr = a.h + row * a.n, *gr = a.gy + row * a.n;
+    double s = 0.0;
+    for (long long i = (long long)threadIdx.x * 4; i < a.n; i += kLongT * 4)
+        s = dot3(load_quad(gr, i, a.n), load_quad(a.weight, i, a.n), load_quad(hr, i, a.n), s);
+    s = block_sum<kLongT>(s, part);
+    const float r = a.rstd[row];
+    const float c = (float)(s / (double)a.n * (double)r * (double)r * (double)r);
+    for (long long i = (long long)threadIdx.x * 4; i < a.n; i += kLongT * 4) {
+        quad_t o = grad_quad(load_quad(hr, i, a.n), load_quad(a.weight, i, a.n), load_quad(gr, i, a.n), r, c);
+        if (a.gh) o += load_quad(a.gh + row * a.n, i, a.n);
+        store_quad(a.gx + row * a.n, i, a.n, o);
+    }
+}
+
+// gw[c] = sum over the G partial rows, in 64 bits: 8 groups of 32 threads take every eighth row each (a quad of columns
+// per thread), and the groups are added in order.
+__global__ __launch_bounds__(256) void rms_norm_grad_fold_kernel(const float *__restrict__ partial, float *__restrict__ gw, long long n, unsigned G)
+{
+    __shared__ double sums[8][32][4];
+    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
+    const long long i = ((long long)blockIdx.x * 32 + lane) * 4;
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    if (i < n)
+#pragma unroll 4
+        for (unsigned b = g; b < G; b += 8) {
+            const quad_t v = load_quad(partial + (size_t)b * n, i, n);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] += (double)v[j];
+        }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums[g][lane][j] = s[j];
+    __syncthreads();
+    if (g == 0 && i < n) {
+        quad_t o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            double t = sums[0][lane][j];
+#pragma unroll
+            for (int k = 1; k < 8; ++k) t += sums[k][lane][j];
+            o[j] = (float)t;
+        }
+        store_quad(gw, i, n, o);
+    }
+}
+
+constexpr int kMaxRegisterRow = 4 * 8 * 1024;
+
+// Blocks that share the rows of a gradient: two per CU, at most one per row.
+inline unsigned norm_grad_blocks(long long rows) { return (unsigned)(rows < 2LL * device_cus() ? rows : 2LL * device_cus()); }
+
+}  // namespace ag
+
+using namespace ag;
+
+extern "C" ag_status_t ag_rms_norm_f32(ag_stream_t stream, const float *x, const float *residual, const float *weight, float eps, float *h,
+                                       float *y, uint8_t *q, uint8_t *scales, float *rstd, int rows, int n)
+{
+    AG_REQUIRE(rows >= 0 && n >= 0, AG_ERR_INVALID_DIMS, "rms_norm: negative extent (%d x %d)", rows, n);
+    AG_REQUIRE(eps >= 0.f, AG_ERR_INVALID_DIMS, "rms_norm: eps (%g) must be a number >= 0", (double)eps);
+    if (rows == 0 || n == 0) return AG_OK;
+    AG_REQUIRE(x && weight, AG_ERR_INVALID_DIMS, "rms_norm: null pointer");
+    AG_REQUIRE((q != nullptr) == (scales != nullptr), AG_ERR_INVALID_DIMS, "rms_norm: 8-bit values and their scales go together");
+    AG_REQUIRE(h || y || q || rstd, AG_ERR_INVALID_DIMS, "rms_norm: no output");
+    AG_REQUIRE(!h || h != y, AG_ERR_INVALID_DIMS, "rms_norm: h and y are the same array");
+    AG_REQUIRE(aligned16(q), AG_ERR_INVALID_DIMS, "rms_norm: 8-bit output must be 16-byte aligned");
+    NormArgs a = {x, residual, weight, h, y, rstd, q, scales, (double)eps, n, (unsigned)(e4m3_pitch(n) / kE4m3Block), (unsigned)e4m3_scale_pitch(n)};
+    hipStream_t st = as_stream(stream);
+    const unsigned R = (unsigned)rows;
+    // Threads of a row: the padding of the scales (a multiple of 512 elements) has to be covered by the quads.
+    const long long cells = (long long)e4m3_scale_pitch(n) * kE4m3Block;
+#define NORM(T, Q) hipLaunchKernelGGL((rms_norm_kernel<T, Q>), dim3(T == 64 ? (R + 3) / 4 : R), dim3(T == 64 ? 256 : T), 0, st, a, R)
+    if (cells <= 512) NORM(64, 2);
+    else if (cells <= 1024) NORM(64, 4);
+    else if (cells <= 2048) NORM(256, 2);
+    else if (cells <= 4096) NORM(256, 4);
+    else if (cells <= 8192) NORM(256, 8);
+    else if (cells <= 16384) NORM(1024, 4);
+    else if (cells <= kMaxRegisterRow) NORM(1024, 8);
+    else hipLaunchKernelGGL(rms_norm_long_kernel, dim3(R), dim3(kLongT), 0, st, a);
+#undef NORM
+    return check_launch("rms_norm");
+}
+
+extern "C" size_t ag_rms_norm_grad_f32_workspace(int rows, int n)
+{
+    if (rows <= 0 || n <= 0) return 0;
+    return (size_t)norm_grad_blocks(rows) * (size_t)n * sizeof(float);
+}
+
+extern "C" ag_status_t ag_rms_norm_grad_f32(ag_stream_t stream, const float *h, const float *weight, const float *rstd, const float *gy,
+                                            const float *gh, float *gx, float *gw, int rows, int n, void *ws, size_t ws_bytes)
+{
+    AG_REQUIRE(rows >= 0 && n >= 0, AG_ERR_INVALID_DIMS, "rms_norm_grad: negative extent (%d x %d)", rows, n);
+    if (n == 0) return AG_OK;
+    hipStream_t st = as_stream(stream);
+    if (rows == 0) {  // no row contributes
+        if (!gw) return AG_OK;
+        return ag_fill_f32(stream, gw, 0.f, (size_t)n);
+    }
+    AG_REQUIRE(h && weight && rstd && gy, AG_ERR_INVALID_DIMS, "rms_norm_grad: null pointer");
+    AG_REQUIRE(gx || gw, AG_ERR_INVALID_DIMS, "rms_norm_grad: no output");
+    AG_REQUIRE(gx != h || !gx, AG_ERR_INVALID_DIMS, "rms_norm_grad: gx must not be h");
+    AG_REQUIRE(!gw || (ws && ws_bytes >= ag_rms_norm_grad_f32_workspace(rows, n)), AG_ERR_INVALID_DIMS,
+               "rms_norm_grad: workspace of %zu bytes, %zu needed", ws_bytes, ag_rms_norm_grad_f32_workspace(rows, n));
+    AG_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 3u) == 0, AG_ERR_INVALID_DIMS, "rms_norm_grad: misaligned workspace");
+    const unsigned R = (unsigned)rows, G = norm_grad_blocks(rows);
+    NormGradArgs a = {h, weight, rstd, gy, gh, gx, gw ? static_cast<float *>(ws) : nullptr, n};
+#define GRAD(T, Q) hipLaunchKernelGGL((rms_norm_grad_kernel<T, Q>), dim3(G), dim3(T), 0, st, a, R)
+    if (n <= 1024) GRAD(256, 1);
+    else if (n <= 2048) GRAD(256, 2);
+    else if (n <= 4096) GRAD(256, 4);
+    else if (n <= 8192) GRAD(512, 4);
+    else if (n <= 16384) GRAD(1024, 4);
+    else {
+        if (gw) hipLaunchKernelGGL(rms_norm_grad_weight_long_kernel, dim3(G, (unsigned)((n + 1023) / 1024)), dim3(256), 0, st, a, R);
+        if (gx) hipLaunchKernelGGL(rms_norm_grad_long_kernel, dim3(R), dim3(kLongT), 0, st, a);
+    }
+#undef GRAD
+    if (gw)
+        hipLaunchKernelGGL(rms_norm_grad_fold_kernel, dim3((unsigned)((n + 127) / 128)), dim3(256), 0, st, static_cast<const float *>(ws), gw, n, G);
+    return check_launch("rms_norm_grad");
+}

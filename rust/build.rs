@@ -8,6 +8,7 @@ use std::{env, path::PathBuf, process::Command};
 
 const SOURCES: &[&str] = &[
     "common", "im2col", "gemm", "gemm_dl", "conv", "conv_s2", "pool", "reduce", "adam", "elementwise",
+    "quantize", "gemm_e4m3", "norm", "clip",
 ];
 
 fn main() {
@@ -27,7 +28,7 @@ fn main() {
         match *name {
             // AdamOp's separately rounded multiplies and adds (gradient_descent_ops/adam.rs:16-50)
             "adam" => { cmd.arg("-ffp-contract=off"); }
-            "gemm_dl" => { cmd.args(["-Wno-inline-asm", "-Wno-pass-failed"]); }
+            "gemm_dl" | "gemm_e4m3" => { cmd.args(["-Wno-inline-asm", "-Wno-pass-failed"]); }
             _ => {}
         }
         cmd.arg(src.join(format!("{name}.hip"))).arg("-o").arg(&object);

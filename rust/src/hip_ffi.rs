@@ -66,6 +66,20 @@ extern "C" {
     pub fn ag_sparse_softmax_xent_f32(stream: AgStream, logits: *const f32, labels: *const f32, loss: *mut f32, log_softmax: *mut f32, rows: usize, classes: usize) -> AgStatus;
     pub fn ag_sparse_softmax_xent_grad_f32(stream: AgStream, log_softmax: *const f32, labels: *const f32, gy: *const f32, gx: *mut f32, rows: usize, classes: usize) -> AgStatus;
     pub fn ag_sparse_softmax_xent_grad_logits_f32(stream: AgStream, logits: *const f32, labels: *const f32, gy: *const f32, gy_const: f32, gx: *mut f32, rows: usize, classes: usize) -> AgStatus;
+    pub fn ag_e4m3_pitch(n: c_int) -> usize;
+    pub fn ag_e4m3_scale_pitch(n: c_int) -> usize;
+    pub fn ag_quantize_e4m3_f32(stream: AgStream, x: *const f32, ldx: c_int, rows: c_int, cols: c_int, q: *mut u8, scales: *mut u8, qt: *mut u8, scales_t: *mut u8) -> AgStatus;
+    pub fn ag_matmul_e4m3_f32_workspace(M: c_int, N: c_int, K: c_int) -> usize;
+    pub fn ag_matmul_e4m3_f32(stream: AgStream, M: c_int, N: c_int, K: c_int, A: *const u8, a_scales: *const u8, B: *const u8, b_scales: *const u8, C: *mut f32, ldc: c_int, ws: *mut c_void, ws_bytes: usize) -> AgStatus;
+    pub fn ag_quantize_matmul_e4m3_f32_workspace(M: c_int, N: c_int, K: c_int) -> usize;
+    pub fn ag_quantize_matmul_e4m3_f32(stream: AgStream, M: c_int, N: c_int, K: c_int, x: *const f32, ldx: c_int, B: *const u8, b_scales: *const u8, C: *mut f32, ldc: c_int, ws: *mut c_void, ws_bytes: usize) -> AgStatus;
+    pub fn ag_rms_norm_f32(stream: AgStream, x: *const f32, residual: *const f32, weight: *const f32, eps: f32, h: *mut f32, y: *mut f32, q: *mut u8, scales: *mut u8, rstd: *mut f32, rows: c_int, n: c_int) -> AgStatus;
+    pub fn ag_rms_norm_grad_f32_workspace(rows: c_int, n: c_int) -> usize;
+    pub fn ag_rms_norm_grad_f32(stream: AgStream, h: *const f32, weight: *const f32, rstd: *const f32, gy: *const f32, gh: *const f32, gx: *mut f32, gw: *mut f32, rows: c_int, n: c_int, ws: *mut c_void, ws_bytes: usize) -> AgStatus;
+    pub fn ag_global_norm_f32_workspace(count: c_int, ns: *const usize) -> usize;
+    pub fn ag_global_norm_f32(stream: AgStream, count: c_int, xs: *const *const f32, ns: *const usize, max_norm: f32, clip: *mut f32, ws: *mut c_void, ws_bytes: usize) -> AgStatus;
+    pub fn ag_clip_by_global_norm_f32(stream: AgStream, count: c_int, xs: *const *const f32, outs: *const *mut f32, ns: *const usize, max_norm: f32, clip: *mut f32, ws: *mut c_void, ws_bytes: usize) -> AgStatus;
+    pub fn ag_adam_update_multi_clipped_f32(stream: AgStream, count: c_int, params: *const *mut f32, grads: *const *const f32, ms: *const *mut f32, vs: *const *mut f32, ts: *const *mut f32, ns: *const usize, alpha: f32, eps: f32, b1: f32, b2: f32, clip: *const f32) -> AgStatus;
     pub fn ag_matmul_f32_static_scratch_bytes() -> usize;
     pub fn ag_matmul_f32_noalloc(stream: AgStream, transA: c_int, transB: c_int, M: c_int, N: c_int, K: c_int, A: *const f32, lda: c_int, B: *const f32, ldb: c_int, C: *mut f32, ldc: c_int) -> AgStatus;
 }
