@@ -79,6 +79,14 @@ int agh_nth_tensor(agh_ctx *ctx, int x, int n);
 int agh_reshape(agh_ctx *ctx, int x, const int64_t *shape, int rank);
 int agh_sparse_softmax_cross_entropy(agh_ctx *ctx, int logits, int labels);
 int agh_stop_gradient(agh_ctx *ctx, int x);
+/* Without counterparts in the reference: the product of two matrices rounded to 8 bits in blocks of 128 along the
+ * contraction (its gradients are products of the same kind), the RMS norm over the last axis (evaluated in one pass with
+ * the sum in front of it), the norm over all elements of n tensors as [norm, clipping coefficient], and the n tensors
+ * times that coefficient (ids to out).  See ag_matmul_e4m3_f32, ag_rms_norm_f32 and ag_clip_by_global_norm_f32. */
+int agh_matmul_e4m3(agh_ctx *ctx, int a, int b, int trans_a, int trans_b);
+int agh_rms_norm(agh_ctx *ctx, int x, int weight, float eps);
+int agh_global_norm(agh_ctx *ctx, const int *xs, int n, float max_norm);
+int agh_clip_by_global_norm(agh_ctx *ctx, const int *xs, int n, float max_norm, int *out);
 /* tensor_ops::grad(ys, xs): writes nx tensor ids to out. */
 int agh_grad(agh_ctx *ctx, const int *ys, int ny, const int *xs, int nx, int *out);
 /* tensor_ops::grad_with_default(ys, xs, ys_grads): ys_grads[i] is the known gradient of ys[i]. */
@@ -107,6 +115,8 @@ agh_adam *agh_adam_new(agh_env *env, const char *adam_ns, const int *var_ids, in
 void agh_adam_free(agh_adam *adam);
 /* Optimizer::get_update_op: one tensor whose evaluation applies every update. */
 int agh_adam_update_op(agh_adam *adam, agh_ctx *ctx, const int *params, const int *grads, int n);
+/* The same with the gradients clipped to max_norm by their norm over all n of them, where the updates read them. */
+int agh_adam_update_op_clipped(agh_adam *adam, agh_ctx *ctx, const int *params, const int *grads, int n, float max_norm);
 
 /* ---- evaluation ----------------------------------------------------------------------------- */
 /* ctx.evaluator().extend(tensors).feed(name, array)...run().  Results stay in the context until

@@ -160,6 +160,7 @@ struct TensorInternal {  // src/tensor.rs:408-441
 struct AdamJob {
     NdArray p, g, m, v, t;
     float alpha, eps, b1, b2;
+    NdArray clip;  // [norm, coefficient] of ag_global_norm_f32; undefined: the gradient as it is
 };
 class DeferredUpdates {
   public:
@@ -234,8 +235,8 @@ class Op {
     virtual void grad(GradientContext &ctx) const = 0;
     // Evaluation-time fusion with the op that produces input 0 (no counterpart in the reference, whose evaluator
     // runs every node on its own, src/evaluation.rs:310-329).  When the evaluator reaches a node whose first input has
-    // not been computed yet and fuses_with_producer(that input's op) holds, it gathers the PRODUCER's inputs instead
-    // and calls compute_with_producer: the op may then write the producer's outputs (`producer_outputs`) and its own
+    // not been computed yet and fuses_with_producer(that input's op) holds, it gathers the PRODUCER's inputs and
+    // behind them the node's own from the second on, and calls compute_with_producer: the op may then write the producer's outputs (`producer_outputs`) and its own
     // (ctx) in one pass and return true, or touch nothing and return false, upon which both nodes are evaluated the
     // ordinary way.  The results must have the bits of the two nodes evaluated in turn.
     virtual bool fuses_with_producer(const Op &) const { return false; }
@@ -319,9 +320,13 @@ class Graph {
     size_t num_nodes() const { return nodes_.size(); }
     Tensor tensor(TensorID id) { return Tensor{this, id}; }
     TensorID install(std::unique_ptr<TensorInternal> n);  // src/graph.rs:27-47 (node-count guards)
+    // The nodes of this graph that round a tensor to 8 bits, by tensor and orientation: products that share an operand
+    // share its rounding.
+    std::map<std::pair<TensorID, int>, TensorID> &rounded_operands() { return rounded_operands_; }
 
   private:
     std::vector<std::unique_ptr<TensorInternal>> nodes_;
+    std::map<std::pair<TensorID, int>, TensorID> rounded_operands_;
 };
 
 class Evaluator;
@@ -385,6 +390,17 @@ Tensor add_n(const std::vector<Tensor> &xs);                                    
 Tensor nth_tensor(Tensor x, int n);                                                       // :545
 Tensor reshape(Tensor x, const Shape &shape);  // one extent may be -1
 Tensor sparse_softmax_cross_entropy(Tensor logits, Tensor labels);
+// Without counterparts in the reference:
+// a . b (each 2-D, transposed where asked) with both operands rounded to 8 bits in blocks of 128 along the contraction
+// (ag_quantize_e4m3_f32), f32 sums; its gradients are products of the same kind, of operands rounded along theirs.  Of an
+// rms_norm's output the 8-bit operand is written by the norm itself.
+Tensor matmul_e4m3(Tensor a, Tensor b, bool trans_a = false, bool trans_b = false);
+// x / sqrt(mean(x^2) + eps) * weight over the last axis.  Where x is a sum of two tensors of one shape (a residual), sum
+// and norm are evaluated in one pass.
+Tensor rms_norm(Tensor x, Tensor weight, float eps);
+// [norm over all elements of the tensors, coefficient that brings it to at most max_norm], and the tensors times it.
+Tensor global_norm(const std::vector<Tensor> &xs, float max_norm);
+std::vector<Tensor> clip_by_global_norm(const std::vector<Tensor> &xs, float max_norm);
 Tensor scalar(float v, Graph *g);
 Tensor zeros_like(Tensor x);      // zeros(shape(x)): what grad() returns for a non-differentiable x
 Tensor stop_gradient(Tensor x);
@@ -412,11 +428,15 @@ class Adam {
     {
         return Adam(0.001f, 1e-08f, 0.9f, 0.999f, vars, env, std::move(adam_namespace_id));
     }
-    std::vector<Tensor> compute_updates(const std::vector<Tensor> &params, const std::vector<Tensor> &grads,
-                                        Context &ctx) const;                                     // adam.rs:116-153
+    // max_norm (no counterpart in the reference): the gradients are clipped to it by their norm over all parameters, where
+    // the updates read them.
+    std::vector<Tensor> compute_updates(const std::vector<Tensor> &params, const std::vector<Tensor> &grads, Context &ctx,
+                                        std::optional<float> max_norm = std::nullopt) const;     // adam.rs:116-153
     void update(const std::vector<Tensor> &params, const std::vector<Tensor> &grads, Context &ctx,
-                const std::vector<std::pair<std::string, NdArray>> &feeds) const;                // mod.rs:66-85
-    Tensor get_update_op(const std::vector<Tensor> &params, const std::vector<Tensor> &grads, Context &ctx) const;
+                const std::vector<std::pair<std::string, NdArray>> &feeds,
+                std::optional<float> max_norm = std::nullopt) const;                             // mod.rs:66-85
+    Tensor get_update_op(const std::vector<Tensor> &params, const std::vector<Tensor> &grads, Context &ctx,
+                         std::optional<float> max_norm = std::nullopt) const;
 
   private:
     float alpha_, eps_, b1_, b2_;

@@ -206,6 +206,37 @@ int agh_sparse_softmax_cross_entropy(agh_ctx *c, int logits, int labels)
     return guard([&] { return tensor_ops::sparse_softmax_cross_entropy(T(c, logits), T(c, labels)).id; });
 }
 
+int agh_matmul_e4m3(agh_ctx *c, int a, int b, int ta, int tb)
+{
+    return guard([&] { return tensor_ops::matmul_e4m3(T(c, a), T(c, b), ta != 0, tb != 0).id; });
+}
+
+int agh_rms_norm(agh_ctx *c, int x, int weight, float eps)
+{
+    return guard([&] { return tensor_ops::rms_norm(T(c, x), T(c, weight), eps).id; });
+}
+
+static std::vector<Tensor> tensors(agh_ctx *c, const int *xs, int n)
+{
+    std::vector<Tensor> ts;
+    for (int i = 0; i < n; ++i) ts.push_back(T(c, xs[i]));
+    return ts;
+}
+
+int agh_global_norm(agh_ctx *c, const int *xs, int n, float max_norm)
+{
+    return guard([&] { return tensor_ops::global_norm(tensors(c, xs, n), max_norm).id; });
+}
+
+int agh_clip_by_global_norm(agh_ctx *c, const int *xs, int n, float max_norm, int *out)
+{
+    return guard([&] {
+        const std::vector<Tensor> r = tensor_ops::clip_by_global_norm(tensors(c, xs, n), max_norm);
+        for (size_t i = 0; i < r.size(); ++i) out[i] = r[i].id;
+        return 0;
+    });
+}
+
 int agh_stop_gradient(agh_ctx *c, int x) { return guard([&] { return tensor_ops::stop_gradient(T(c, x)).id; }); }
 
 int agh_grad(agh_ctx *c, const int *ys, int ny, const int *xs, int nx, int *out)
@@ -293,6 +324,11 @@ int agh_adam_update_op(agh_adam *adam, agh_ctx *c, const int *params, const int 
         }
         return adam->adam.get_update_op(p, g, c->ctx).id;
     });
+}
+
+int agh_adam_update_op_clipped(agh_adam *adam, agh_ctx *c, const int *params, const int *grads, int n, float max_norm)
+{
+    return guard([&] { return adam->adam.get_update_op(tensors(c, params, n), tensors(c, grads, n), c->ctx, max_norm).id; });
 }
 
 static int eval_impl(agh_ctx *c, const int *tensors, int n, const char *const *feed_names, const float *const *feed_data,

@@ -1386,7 +1386,8 @@ struct SparseSoftmaxCrossEntropy : Op {  // xent_ops.rs:63-137
 // ------------------------------------------------------------------------------------------
 struct AdamOp : Op {
     float alpha, eps, b1, b2;
-    AdamOp(float a, float e, float x, float y) : alpha(a), eps(e), b1(x), b2(y) {}
+    bool clipped;  // input 5: the clipping coefficient (a GlobalNorm node)
+    AdamOp(float a, float e, float x, float y, bool c) : alpha(a), eps(e), b1(x), b2(y), clipped(c) {}
     const char *name() const override { return "AdamOp"; }
     OpError compute(ComputeContext &ctx) const override
     {
@@ -1396,15 +1397,275 @@ struct AdamOp : Op {
         if (g.len() != p.len() || m.len() != p.len() || v.len() != p.len())
             return OpError::make(ErrorKind::IncompatibleShape, "AdamOp: parameter, gradient and moment shapes differ");
         if (t.len() < 1) return OpError::make(ErrorKind::IncompatibleShape, "AdamOp: empty step counter");
-        ctx.adam_update(AdamJob{p, g, m, v, t, alpha, eps, b1, b2});
+        ctx.adam_update(AdamJob{p, g, m, v, t, alpha, eps, b1, b2, clipped ? ctx.input(5) : NdArray()});
         ctx.append_empty_output();
         return OpError::none();
     }
     void grad(GradientContext &ctx) const override
     {
-        for (int i = 0; i < 5; ++i) ctx.append_input_grad(std::nullopt);
+        for (size_t i = 0; i < ctx.num_inputs(); ++i) ctx.append_input_grad(std::nullopt);
     }
 };
+
+// ------------------------------------------------------------------------------------------
+// 8-bit products, RMS norm, clipping (no counterparts in the reference)
+// ------------------------------------------------------------------------------------------
+// Both extents of a matrix as the kernels take them.
+OpError matrix_extents(const char *who, const Shape &s, int *rows, int *cols)
+{
+    if (s.size() != 2) return OpError::make(ErrorKind::IncompatibleShape, std::string(who) + ": operand must be 2D (got " + shape_str(s) + ")");
+    if (s[0] > 0x7fffffff || s[1] > 0x7fffffff) return OpError::make(ErrorKind::InvalidDims, std::string(who) + ": extents " + shape_str(s));
+    *rows = (int)s[0];
+    *cols = (int)s[1];
+    return OpError::none();
+}
+
+// Bytes of an 8-bit operand, four to an element of the array.
+NdArray operand_values(int rows, int n) { return NdArray::empty({(int64_t)((size_t)rows * ag_e4m3_pitch(n) / 4)}); }
+NdArray operand_scales(int rows, int n) { return NdArray::empty({(int64_t)((size_t)rows * ag_e4m3_scale_pitch(n) / 4)}); }
+uint8_t *bytes(const NdArray &a) { return reinterpret_cast<uint8_t *>(a.ptr()); }
+
+// A matrix rounded to 8 bits along its rows and / or columns: outputs values and scales of the orientations it was built
+// for, rows first.
+struct QuantizeE4m3 : Op {
+    enum Orientation { Rows = 1, Columns = 2 };
+    int orientation;
+    explicit QuantizeE4m3(int o) : orientation(o) {}
+    const char *name() const override { return "QuantizeE4m3"; }
+    OpError compute(ComputeContext &ctx) const override
+    {
+        const NdArray x = ctx.input(0);
+        int rows, cols;
+        OpError e = matrix_extents("matmul_e4m3", x.shape(), &rows, &cols);
+        if (!e.ok()) return e;
+        NdArray q, s, qt, st;
+        if (orientation & Rows) q = operand_values(rows, cols), s = operand_scales(rows, cols);
+        if (orientation & Columns) qt = operand_values(cols, rows), st = operand_scales(cols, rows);
+        e = from_status(ag_quantize_e4m3_f32(ctx.stream(), x.ptr(), cols, rows, cols, bytes(q), bytes(s), bytes(qt), bytes(st)));
+        if (!e.ok()) return e;
+        if (orientation & Rows) {
+            ctx.append_output(q);
+            ctx.append_output(s);
+        }
+        if (orientation & Columns) {
+            ctx.append_output(qt);
+            ctx.append_output(st);
+        }
+        return OpError::none();
+    }
+    // (the product's back-prop inputs are the tensors themselves: nothing differentiates through the rounding)
+    void grad(GradientContext &ctx) const override { ctx.append_input_grad(std::nullopt); }
+};
+
+// Inputs: values and scales of either operand, then the extents of the two tensors they were rounded from; the back-prop
+// inputs are those two tensors.
+struct MatMulE4m3 : Op {
+    bool transpose_a, transpose_b;
+    TensorID a, b;
+    MatMulE4m3(bool ta, bool tb, TensorID ia, TensorID ib) : transpose_a(ta), transpose_b(tb), a(ia), b(ib) {}
+    const char *name() const override { return "MatMulE4m3"; }
+    OpError compute(ComputeContext &ctx) const override
+    {
+        int ar, ac, br, bc;
+        OpError e = matrix_extents("matmul_e4m3", ctx.input_shape(4), &ar, &ac);
+        if (e.ok()) e = matrix_extents("matmul_e4m3", ctx.input_shape(5), &br, &bc);
+        if (!e.ok()) return e;
+        const int m = transpose_a ? ac : ar, k = transpose_a ? ar : ac, k2 = transpose_b ? bc : br, n = transpose_b ? br : bc;
+        if (k != k2)
+            return OpError::make(ErrorKind::IncompatibleShape, "matmul_e4m3: inputs " + std::to_string(m) + " \xc3\x97 " + std::to_string(k) + " and " +
+                                                                   std::to_string(k2) + " \xc3\x97 " + std::to_string(n));
+        const NdArray qa = ctx.input(0), sa = ctx.input(1), qb = ctx.input(2), sb = ctx.input(3);
+        NdArray c = NdArray::empty({m, n});
+        const size_t need = ag_matmul_e4m3_f32_workspace(m, n, k);
+        NdArray ws;
+        if (need) ws = workspace(need);
+        e = from_status(ag_matmul_e4m3_f32(ctx.stream(), m, n, k, bytes(qa), bytes(sa), bytes(qb), bytes(sb), c.ptr(), std::max(n, 1),
+                                           need ? ws.ptr() : nullptr, need));
+        if (!e.ok()) return e;
+        ctx.append_output(c);
+        return OpError::none();
+    }
+    void grad(GradientContext &ctx) const override;
+};
+
+struct RmsNormGrad : Op {  // inputs x, weight, rstd, gy; outputs gx, gw
+    const char *name() const override { return "RmsNormGrad"; }
+    OpError compute(ComputeContext &ctx) const override
+    {
+        const NdArray x = ctx.input(0), w = ctx.input(1), rstd = ctx.input(2), gy = ctx.input(3);
+        if (gy.shape() != x.shape()) return OpError::make(ErrorKind::IncompatibleShape, "rms_norm grad: shapes differ");
+        const int n = (int)x.shape().back(), rows = n ? (int)(x.len() / (size_t)n) : 0;
+        NdArray gx = NdArray::empty(x.shape()), gw = NdArray::empty(w.shape());
+        NdArray ws = workspace(ag_rms_norm_grad_f32_workspace(rows, n));
+        const OpError e = from_status(ag_rms_norm_grad_f32(ctx.stream(), x.ptr(), w.ptr(), rstd.ptr(), gy.ptr(), nullptr, gx.ptr(), gw.ptr(), rows, n,
+                                                           ws.ptr(), ws.len() * 4));
+        if (!e.ok()) return e;
+        ctx.append_output(gx);
+        ctx.append_output(gw);
+        return OpError::none();
+    }
+    void grad(GradientContext &) const override { throw Panic("rms_norm: there is no second-order gradient"); }
+};
+
+// Inputs x, weight; outputs y, rstd and, once an 8-bit product reads y, y's values and scales rounded along its rows.
+struct RmsNorm : Op {
+    float eps;
+    bool emit_e4m3 = false;  // set by tensor_ops::matmul_e4m3
+    explicit RmsNorm(float e) : eps(e) {}
+    const char *name() const override { return "RmsNorm"; }
+    // x + residual (residual may be undefined) and its norm; `h`: the sum.
+    OpError run(ComputeContext &ctx, const NdArray &x, const NdArray &residual, const NdArray &w, const NdArray &h) const
+    {
+        if (x.ndim() < 1 || w.ndim() != 1 || w.shape()[0] != x.shape().back())
+            return OpError::make(ErrorKind::IncompatibleShape, "rms_norm: weight " + shape_str(w.shape()) + " for rows of " + shape_str(x.shape()));
+        const int64_t n = x.shape().back(), rows = n ? (int64_t)(x.len() / (size_t)n) : 0;
+        if (n > 0x7fffffff || rows > 0x7fffffff) return OpError::make(ErrorKind::InvalidDims, "rms_norm: extents " + shape_str(x.shape()));
+        NdArray y = NdArray::empty(x.shape()), rstd = NdArray::empty({rows}), q, s;
+        if (emit_e4m3) q = operand_values((int)rows, (int)n), s = operand_scales((int)rows, (int)n);
+        const OpError e = from_status(ag_rms_norm_f32(ctx.stream(), x.ptr(), residual.defined() ? residual.ptr() : nullptr, w.ptr(), eps,
+                                                      h.defined() ? h.ptr() : nullptr, y.ptr(), emit_e4m3 ? bytes(q) : nullptr,
+                                                      emit_e4m3 ? bytes(s) : nullptr, rstd.ptr(), (int)rows, (int)n));
+        if (!e.ok()) return e;
+        ctx.append_output(y);
+        ctx.append_output(rstd);
+        if (emit_e4m3) {
+            ctx.append_output(q);
+            ctx.append_output(s);
+        }
+        return OpError::none();
+    }
+    OpError compute(ComputeContext &ctx) const override
+    {
+        const NdArray x = ctx.input(0), w = ctx.input(1);
+        return run(ctx, x, NdArray(), w, NdArray());
+    }
+    // The sum of two tensors of one shape in front of the norm: one pass writes the sum and norms it.
+    bool fuses_with_producer(const Op &producer) const override { return dynamic_cast<const AddOp *>(&producer) != nullptr; }
+    bool compute_with_producer(ComputeContext &ctx, const Op &, std::vector<NdArray> *producer_outputs, OpError *status) const override
+    {
+        if (ctx.num_inputs() != 3 || ctx.input_shape(0) != ctx.input_shape(1) || ctx.input_shape(0).empty()) return false;
+        for (int64_t d : ctx.input_shape(0))
+            if (d == 0) return false;
+        if (ctx.input_shape(2).size() != 1 || ctx.input_shape(2)[0] != ctx.input_shape(0).back()) return false;
+        const NdArray a = ctx.input(0), b = ctx.input(1), w = ctx.input(2);
+        const NdArray h = NdArray::empty(a.shape());
+        *status = run(ctx, a, b, w, h);
+        if (status->ok()) producer_outputs->push_back(h);
+        return true;
+    }
+    void grad(GradientContext &ctx) const override
+    {
+        const Tensor both = ctx.graph()
+                                ->builder()
+                                .append_input(ctx.input(0), false)
+                                .append_input(ctx.input(1), false)
+                                .append_input_with_selector(ctx.output(), false, 1)
+                                .append_input(ctx.output_grad(), false)
+                                .build(std::make_unique<RmsNormGrad>());
+        ctx.append_input_grad(both);
+        ctx.append_input_grad(tensor_ops::nth_tensor(both, 1));
+    }
+};
+
+// The tensor's node rounded for one side of a product: the node and the selector of its values (the scales come next).
+struct RoundedOperand {
+    Tensor node;
+    int values;
+};
+
+RoundedOperand rounded_operand(Tensor x, bool rows)
+{
+    Graph *g = x.graph;
+    if (auto *norm = dynamic_cast<RmsNorm *>(g->node(x.id).op.get()); norm && rows) {
+        norm->emit_e4m3 = true;
+        return {x, 2};
+    }
+    const int want = rows ? QuantizeE4m3::Rows : QuantizeE4m3::Columns;
+    auto &known = g->rounded_operands();
+    if (auto it = known.find({x.id, QuantizeE4m3::Rows | QuantizeE4m3::Columns}); it != known.end()) return {g->tensor(it->second), rows ? 0 : 2};
+    if (auto it = known.find({x.id, want}); it != known.end()) return {g->tensor(it->second), 0};
+    const Tensor t = build(g, {x}, std::make_unique<QuantizeE4m3>(want));
+    known[{x.id, want}] = t.id;
+    return {t, 0};
+}
+
+void MatMulE4m3::grad(GradientContext &ctx) const
+{
+    // y = op(a) op(b): the gradient of op(a) is gy op(b)^T, that of op(b) op(a)^T gy.  gy enters the first along its rows
+    // and the second along its columns: one node rounds both ways.
+    Graph *g = ctx.graph();
+    const Tensor gy = ctx.output_grad(), ta = g->tensor(a), tb = g->tensor(b);
+    const int both = QuantizeE4m3::Rows | QuantizeE4m3::Columns;
+    if (g->rounded_operands().count({gy.id, both}) == 0)
+        g->rounded_operands()[{gy.id, both}] = build(g, {gy}, std::make_unique<QuantizeE4m3>(both)).id;
+    ctx.append_input_grad(transpose_a ? tensor_ops::matmul_e4m3(tb, gy, transpose_b, true) : tensor_ops::matmul_e4m3(gy, tb, false, !transpose_b));
+    ctx.append_input_grad(transpose_b ? tensor_ops::matmul_e4m3(gy, ta, true, transpose_a) : tensor_ops::matmul_e4m3(ta, gy, !transpose_a, false));
+}
+
+// [norm, coefficient] over all inputs.
+struct GlobalNorm : Op {
+    float max_norm;
+    explicit GlobalNorm(float m) : max_norm(m) {}
+    const char *name() const override { return "GlobalNorm"; }
+    OpError compute(ComputeContext &ctx) const override
+    {
+        std::vector<NdArray> xs;
+        std::vector<const float *> px;
+        std::vector<size_t> ns;
+        for (size_t i = 0; i < ctx.num_inputs(); ++i) {
+            xs.push_back(ctx.input(i));
+            px.push_back(xs.back().ptr());
+            ns.push_back(xs.back().len());
+        }
+        NdArray clip = NdArray::empty({2});
+        NdArray ws = workspace(ag_global_norm_f32_workspace((int)ns.size(), ns.data()));
+        const OpError e = from_status(ag_global_norm_f32(ctx.stream(), (int)ns.size(), px.data(), ns.data(), max_norm, clip.ptr(), ws.ptr(), ws.len() * 4));
+        if (!e.ok()) return e;
+        ctx.append_output(clip);
+        return OpError::none();
+    }
+    void grad(GradientContext &) const override { throw Panic("global_norm: there is no gradient"); }
+};
+
+// Outputs: [norm, coefficient], then every input times the coefficient.
+struct ClipByGlobalNorm : Op {
+    float max_norm;
+    explicit ClipByGlobalNorm(float m) : max_norm(m) {}
+    const char *name() const override { return "ClipByGlobalNorm"; }
+    OpError compute(ComputeContext &ctx) const override
+    {
+        std::vector<NdArray> xs, outs;
+        std::vector<const float *> px;
+        std::vector<float *> po;
+        std::vector<size_t> ns;
+        for (size_t i = 0; i < ctx.num_inputs(); ++i) {
+            xs.push_back(ctx.input(i));
+            outs.push_back(NdArray::empty(xs.back().shape()));
+            px.push_back(xs.back().ptr());
+            po.push_back(outs.back().ptr());
+            ns.push_back(xs.back().len());
+        }
+        NdArray clip = NdArray::empty({2});
+        NdArray ws = workspace(ag_global_norm_f32_workspace((int)ns.size(), ns.data()));
+        const OpError e = from_status(
+            ag_clip_by_global_norm_f32(ctx.stream(), (int)ns.size(), px.data(), po.data(), ns.data(), max_norm, clip.ptr(), ws.ptr(), ws.len() * 4));
+        if (!e.ok()) return e;
+        ctx.append_output(clip);
+        for (const NdArray &o : outs) ctx.append_output(o);
+        return OpError::none();
+    }
+    void grad(GradientContext &) const override { throw Panic("clip_by_global_norm: there is no gradient"); }
+};
+
+template <typename NormOp>
+Tensor over_all(const char *who, const std::vector<Tensor> &xs, float max_norm)
+{
+    if (xs.empty()) throw Panic(std::string(who) + ": no tensors");
+    if (!(max_norm >= 0.f)) throw Panic(std::string(who) + ": max_norm must be a number >= 0");
+    TensorBuilder b = xs[0].graph->builder();
+    for (const Tensor &t : xs) b.append_input(t, false);
+    return b.build(std::make_unique<NormOp>(max_norm));
+}
 
 }  // namespace
 
@@ -1490,6 +1751,39 @@ Tensor sparse_softmax_cross_entropy(Tensor logits, Tensor labels)
     return build(logits.graph, {logits, labels}, std::make_unique<SparseSoftmaxCrossEntropy>());
 }
 
+Tensor matmul_e4m3(Tensor a, Tensor b, bool trans_a, bool trans_b)
+{
+    if (a.graph != b.graph) throw Panic("Detected tensors belonging to different graphs");
+    // the left operand's rows run along the contraction unless it is transposed, the right one's if it is
+    const RoundedOperand qa = rounded_operand(a, !trans_a), qb = rounded_operand(b, trans_b);
+    return a.graph->builder()
+        .append_input_with_selector(qa.node, false, qa.values)
+        .append_input_with_selector(qa.node, false, qa.values + 1)
+        .append_input_with_selector(qb.node, false, qb.values)
+        .append_input_with_selector(qb.node, false, qb.values + 1)
+        .append_input(extents_of(a), false)
+        .append_input(extents_of(b), false)
+        .append_backprop_input(a)
+        .append_backprop_input(b)
+        .build(std::make_unique<MatMulE4m3>(trans_a, trans_b, a.id, b.id));
+}
+
+Tensor rms_norm(Tensor x, Tensor weight, float eps)
+{
+    if (!(eps >= 0.f)) throw Panic("rms_norm: eps must be a number >= 0");
+    return build(x.graph, {x, weight}, std::make_unique<RmsNorm>(eps));
+}
+
+Tensor global_norm(const std::vector<Tensor> &xs, float max_norm) { return over_all<GlobalNorm>("global_norm", xs, max_norm); }
+
+std::vector<Tensor> clip_by_global_norm(const std::vector<Tensor> &xs, float max_norm)
+{
+    const Tensor all = over_all<ClipByGlobalNorm>("clip_by_global_norm", xs, max_norm);
+    std::vector<Tensor> ret;
+    for (size_t i = 0; i < xs.size(); ++i) ret.push_back(nth_tensor(all, (int)i + 1));
+    return ret;
+}
+
 Tensor scalar(float v, Graph *g) { return g->builder().set_known_shape(Shape{}).build(std::make_unique<ScalarOp>(v)); }
 
 Tensor zeros_like(Tensor x)
@@ -1521,39 +1815,39 @@ Adam::Adam(float alpha, float eps, float b1, float b2, const std::vector<Variabl
     }
 }
 
-std::vector<Tensor> Adam::compute_updates(const std::vector<Tensor> &params, const std::vector<Tensor> &grads,
-                                          Context &ctx) const
+std::vector<Tensor> Adam::compute_updates(const std::vector<Tensor> &params, const std::vector<Tensor> &grads, Context &ctx,
+                                          std::optional<float> max_norm) const
 {
     if (params.size() != grads.size()) throw Panic("assertion failed: num_params == grads.len()");
     std::vector<Tensor> ret;
+    Tensor clip;
+    if (max_norm && !grads.empty()) clip = tensor_ops::global_norm(grads, *max_norm);
     for (size_t i = 0; i < params.size(); ++i) {
         const VariableID vid = ctx.node(params[i].id).variable_id;
         if (vid < 0) throw Panic("Got non-variable tensor");
         const Tensor m = ctx.variable(std::to_string(vid) + "m", ns_);
         const Tensor v = ctx.variable(std::to_string(vid) + "v", ns_);
         const Tensor t = ctx.variable(std::to_string(vid) + "t", ns_);
-        ret.push_back(ctx.builder()
-                          .append_input(params[i], true)
-                          .append_input(grads[i], false)
-                          .append_input(m, true)
-                          .append_input(v, true)
-                          .append_input(t, true)
-                          .build(std::make_unique<AdamOp>(alpha_, eps_, b1_, b2_)));
+        TensorBuilder b = ctx.builder();
+        b.append_input(params[i], true).append_input(grads[i], false).append_input(m, true).append_input(v, true).append_input(t, true);
+        if (clip.valid()) b.append_input(clip, false);
+        ret.push_back(b.build(std::make_unique<AdamOp>(alpha_, eps_, b1_, b2_, clip.valid())));
     }
     return ret;
 }
 
 void Adam::update(const std::vector<Tensor> &params, const std::vector<Tensor> &grads, Context &ctx,
-                  const std::vector<std::pair<std::string, NdArray>> &feeds) const
+                  const std::vector<std::pair<std::string, NdArray>> &feeds, std::optional<float> max_norm) const
 {
-    const std::vector<Tensor> ops = compute_updates(params, grads, ctx);
+    const std::vector<Tensor> ops = compute_updates(params, grads, ctx, max_norm);
     for (const EvalResult &r : ctx.eval(ops, feeds))
         if (!r.error.ok()) throw Panic("called `Result::unwrap()` on an `Err` value: " + r.error.message);
 }
 
-Tensor Adam::get_update_op(const std::vector<Tensor> &params, const std::vector<Tensor> &grads, Context &ctx) const
+Tensor Adam::get_update_op(const std::vector<Tensor> &params, const std::vector<Tensor> &grads, Context &ctx,
+                           std::optional<float> max_norm) const
 {
-    return tensor_ops::add_n(compute_updates(params, grads, ctx));
+    return tensor_ops::add_n(compute_updates(params, grads, ctx, max_norm));
 }
 
 }  // namespace optimizers

@@ -510,6 +510,7 @@ void DeferredUpdates::add(AdamJob job)
         // another optimizer's coefficients, or a gradient that the batch is about to overwrite / a
         // parameter that the batch still reads as a gradient
         clash |= j.alpha != job.alpha || j.eps != job.eps || j.b1 != job.b1 || j.b2 != job.b2;
+        clash |= j.clip.allocation() != job.clip.allocation();
         clash |= job.p.allocation() == j.g.allocation() || job.m.allocation() == j.g.allocation() ||
                  job.v.allocation() == j.g.allocation() || job.t.allocation() == j.g.allocation();
     }
@@ -533,8 +534,11 @@ void DeferredUpdates::flush()
         n.push_back(j.p.len());
     }
     const AdamJob &h = jobs_.front();
-    const ag_status_t st = ag_adam_update_multi_f32(current_stream(), (int)jobs_.size(), p.data(), g.data(), m.data(),
-                                                    v.data(), t.data(), n.data(), h.alpha, h.eps, h.b1, h.b2);
+    const ag_status_t st =
+        h.clip.defined() ? ag_adam_update_multi_clipped_f32(current_stream(), (int)jobs_.size(), p.data(), g.data(), m.data(), v.data(),
+                                                            t.data(), n.data(), h.alpha, h.eps, h.b1, h.b2, h.clip.ptr())
+                         : ag_adam_update_multi_f32(current_stream(), (int)jobs_.size(), p.data(), g.data(), m.data(), v.data(), t.data(),
+                                                    n.data(), h.alpha, h.eps, h.b1, h.b2);
     jobs_.clear();
     if (st != AG_OK) throw std::runtime_error(ag_last_error());
 }
@@ -735,9 +739,10 @@ std::vector<EvalResult> Context::eval(const std::vector<Tensor> &tensors,
     }
     // Inputs of a node, from the feeds, the environment and what has been computed; the first error among them
     // is the node's own (src/evaluation.rs:283-309).
-    auto gather = [&](const TensorInternal &n, std::vector<ComputeContext::Input> *inputs) {
+    auto gather = [&](const TensorInternal &n, std::vector<ComputeContext::Input> *inputs, size_t first = 0) {
         OpError status;
-        for (const IncomingTensor &in : n.incoming_nodes) {
+        for (size_t at = first; at < n.incoming_nodes.size(); ++at) {
+            const IncomingTensor &in = n.incoming_nodes[at];
             const TensorInternal &src = node(in.id);
             if (src.is_placeholder) {
                 inputs->push_back({*find_placeholder(feeds, src), ComputeContext::InputKind::NonVariable});
@@ -791,6 +796,11 @@ std::vector<EvalResult> Context::eval(const std::vector<Tensor> &tensors,
         if (p.is_placeholder || p.is_variable() || !p.op || !n.op->fuses_with_producer(*p.op)) return nullptr;
         for (const IncomingTensor &in : p.incoming_nodes)
             if (in.allow_mut) return nullptr;
+        // The node's other inputs are gathered along with the producer's: sources only, which cannot depend on the producer.
+        for (size_t i = 1; i < n.incoming_nodes.size(); ++i) {
+            const TensorInternal &src = node(n.incoming_nodes[i].id);
+            if (n.incoming_nodes[i].allow_mut || !(src.is_placeholder || src.is_variable())) return nullptr;
+        }
         return &p;
     };
     // Which of the nodes this evaluation will reach are such producers, and of which node: whoever asks for the
@@ -828,6 +838,7 @@ std::vector<EvalResult> Context::eval(const std::vector<Tensor> &tensors,
                 // below has put in front of this node)
                 std::vector<ComputeContext::Input> inputs;
                 OpError status = gather(*p, &inputs);
+                if (status.ok()) status = gather(n, &inputs, 1);
                 bool fused = false;
                 if (status.ok()) {
                     flush_if_touched(inputs);

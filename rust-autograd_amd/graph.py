@@ -55,6 +55,10 @@ PROTOTYPES = {
     "agh_nth_tensor": (_i, [_p, _i, _i]),
     "agh_reshape": (_i, [_p, _i, _lp, _i]),
     "agh_sparse_softmax_cross_entropy": (_i, [_p, _i, _i]),
+    "agh_matmul_e4m3": (_i, [_p, _i, _i, _i, _i]),
+    "agh_rms_norm": (_i, [_p, _i, _i, _f]),
+    "agh_global_norm": (_i, [_p, _ip, _i, _f]),
+    "agh_clip_by_global_norm": (_i, [_p, _ip, _i, _f, _ip]),
     "agh_stop_gradient": (_i, [_p, _i]),
     "agh_grad": (_i, [_p, _ip, _i, _ip, _i, _ip]),
     "agh_grad_with_default": (_i, [_p, _ip, _ip, _i, _ip, _i, _ip]),
@@ -69,6 +73,7 @@ PROTOTYPES = {
     "agh_adam_new": (_p, [_p, _s, _ip, _i, _f, _f, _f, _f]),
     "agh_adam_free": (None, [_p]),
     "agh_adam_update_op": (_i, [_p, _p, _ip, _ip, _i]),
+    "agh_adam_update_op_clipped": (_i, [_p, _p, _ip, _ip, _i, _f]),
     "agh_eval": (_i, [_p, _ip, _i, C.POINTER(_s), C.POINTER(_fp), C.POINTER(_lp), _ip, _i]),
     "agh_eval_nowait": (_i, [_p, _ip, _i, C.POINTER(_s), C.POINTER(_fp), C.POINTER(_lp), _ip, _i]),
     "agh_synchronize": (_i, []),
@@ -317,6 +322,27 @@ class Context:
     def sparse_softmax_cross_entropy(self, logits, labels):
         return self._t(lib().agh_sparse_softmax_cross_entropy(self._h, logits.id, labels.id))
 
+    def matmul_e4m3(self, a, b, trans_a=False, trans_b=False):
+        """a . b with both operands rounded to 8 bits (e4m3, a power of two per block of 128 along the contraction); the
+        gradients are products of the same kind."""
+        return self._t(lib().agh_matmul_e4m3(self._h, a.id, b.id, int(trans_a), int(trans_b)))
+
+    def rms_norm(self, x, weight, eps=1e-6):
+        """x / sqrt(mean(x^2) + eps) * weight over the last axis; a sum in front of it is evaluated in the same pass."""
+        return self._t(lib().agh_rms_norm(self._h, x.id, weight.id, float(eps)))
+
+    def global_norm(self, xs, max_norm=float("inf")):
+        """[norm over all elements of the tensors, the coefficient that clips it to max_norm]."""
+        ids, n = _ints(t.id for t in xs)
+        return self._t(lib().agh_global_norm(self._h, ids, n, float(max_norm)))
+
+    def clip_by_global_norm(self, xs, max_norm):
+        """The tensors times the coefficient that brings their norm over all elements to at most max_norm."""
+        ids, n = _ints(t.id for t in xs)
+        out = (C.c_int * max(n, 1))()
+        _check(lib().agh_clip_by_global_norm(self._h, ids, n, float(max_norm), out))
+        return [self._t(out[i]) for i in range(n)]
+
     def stop_gradient(self, x):
         return self._t(lib().agh_stop_gradient(self._h, x.id))
 
@@ -421,13 +447,16 @@ class Adam:
             _LIB.agh_adam_free(self._h)
             self._h = None
 
-    def get_update_op(self, params, grads, ctx):
+    def get_update_op(self, params, grads, ctx, max_norm=None):
+        """max_norm: the gradients are clipped to it by their norm over all parameters, where the updates read them."""
         pi, n = _ints(t.id for t in params)
         gi, _ = _ints(t.id for t in grads)
+        if max_norm is not None:
+            return ctx._t(lib().agh_adam_update_op_clipped(self._h, ctx._h, pi, gi, n, float(max_norm)))
         return ctx._t(lib().agh_adam_update_op(self._h, ctx._h, pi, gi, n))
 
-    def update(self, params, grads, ctx, feeds=None):
+    def update(self, params, grads, ctx, feeds=None, max_norm=None):
         """Optimizer::update (optimizers/mod.rs:63-81): runs the updates; the call does not wait for the device."""
-        r = ctx.run([self.get_update_op(params, grads, ctx)], feeds)[0]
+        r = ctx.run([self.get_update_op(params, grads, ctx, max_norm)], feeds)[0]
         if isinstance(r, OpError):
             raise r
