@@ -7,6 +7,8 @@
 // would multiply twice as fast, but it does not keep f32 sums: it aligns each group of 8 products to the largest of them
 // and drops what lies 2^-14 below (measured: +2^16 - 2^16 + 2^2 within a group gives 0), 1.4e-5 of the result for
 // Gaussian operands and 6e-5 for wider ones, whatever the length; the bf16 instruction gives 8e-8 and 4e-7.
+#include <type_traits>
+
 #include "e4m3.h"
 
 namespace ag {
@@ -59,17 +61,26 @@ __device__ inline const unsigned char *uniform(const unsigned char *p)
 }
 
 // BM x BN of C per block, WM x WN per wave, 128 of the contraction per step.  LDS holds two steps of both operands, rows of
-// 128 bytes; the 16-byte piece c of row r stands at place c ^ (r & 7), so that the 32 rows that a half wave reads at one
-// piece fall on all banks.  A step's loads are issued at the start of the step before it, behind the barrier that ends
-// the reads of that buffer; its scales come four steps at a time (one word per row), in a second pair of buffers.
+// 128 bytes, and a word of scales per row (four blocks, one of which the step uses).  The 16-byte piece c of row r stands
+// at place c ^ (r & 7) ^ ((r >> 3) & 1), so that 16 consecutive rows read at one piece fall on all 64 banks.
+//
+// What bounds it is power: with Gaussian operands the chip holds the matrix instruction alone, fed from registers, at
+// 1830 TFLOP/s (1.75 GHz; 2480 with zeros), and lowers its clock as the rest of the loop gets out of the way.  4096^3
+// takes 97 us (1415 TFLOP/s), 16384 x 8192 x 8192 1.44-1.46 ms (1500-1530; a bf16 product of the library, from operands
+// twice the size, 1.32 ms), the matrix unit busy for 83 % of the time.  What brought it there, at 4096^3 and at
+// 16384 x 8192 x 8192: every load of a step issued behind the barrier and operands widened where they are used 104 us,
+// 1.61 ms; the next group's operands widened between the instructions of the current one, LDS read a chunk ahead and the
+// barrier in front of a step's last chunk 101 us, 1.48 ms; one basic block per step (no tests around the loads) and the
+// loads spread over four groups 97 us, 1.44 ms.  Four waves of 128 x 128 need a third less of LDS and widening but stand
+// still together: 99 us, 1.46 ms; loads spread singly between the instructions 100 us, 1.48 ms.
 template <int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void gemm_e4m3_tile_kernel(GemmE4m3 p)
 {
     constexpr int WAVES_N = BN / WN, NW = BM / WM * WAVES_N, MI = WM / 32, NI = WN / 32;
     constexpr int ROWS = BM + BN, STEP = ROWS * 128;
-    constexpr int LOADS = ROWS / 8 / NW;  // 1 KiB loads (8 rows) of a wave per step
-    constexpr int SCALE_LOADS = ROWS / 64;
-    static_assert(ROWS % (8 * NW) == 0 && BM % 64 == 0 && BN % 64 == 0 && SCALE_LOADS <= NW, "rows divide over the waves");
+    constexpr int LOADS = ROWS / 8 / NW;         // 1 KiB loads (8 rows) of a wave per step
+    constexpr int SCALE_LOADS = ROWS / 64 / NW;  // 64 words of a wave per step
+    static_assert(ROWS % (8 * NW) == 0 && BM % 64 == 0 && BN % 64 == 0 && ROWS % (64 * NW) == 0, "rows divide over the waves");
     __shared__ __attribute__((aligned(1024))) unsigned char tile[2 * STEP];
     __shared__ __attribute__((aligned(256))) unsigned scale_words[2][ROWS];
     const unsigned lds = (unsigned)(size_t)(lds_byte_t *)tile, lds_scales = (unsigned)(size_t)(lds_byte_t *)scale_words;
@@ -97,69 +108,124 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void gemm_e4m3_tile_kerne
         const int start = min(first, last), row = min(first + (lane >> 3), last);
         base[i] = uniform((in_a ? p.a : p.b) + start * p.pitch);
         // (a row's pitch is at most 2^31: 8 rows pass 32 bits only where one row is longer than 2^28, which the host refuses)
-        offset[i] = (unsigned)((row - start) * p.pitch) + (unsigned)(((lane & 7) ^ (lane >> 3)) * 16);
+        offset[i] = (unsigned)((row - start) * p.pitch) + (unsigned)(((lane & 7) ^ (lane >> 3) ^ ((i * NW + wave) & 1)) * 16);
     }
-    const unsigned char *scale_base = nullptr;
-    unsigned scale_offset = 0;
-    if (wave < SCALE_LOADS) {
-        const int r0 = wave * 64;
+    const unsigned char *scale_base[SCALE_LOADS];
+    unsigned scale_offset[SCALE_LOADS];
+#pragma unroll
+    for (int i = 0; i < SCALE_LOADS; ++i) {
+        const int r0 = (i * NW + wave) * 64;
         const bool in_a = r0 < BM;
         const int first = in_a ? m0 + r0 : n0 + r0 - BM, last = (in_a ? p.M : p.N) - 1;
         const int start = min(first, last), row = min(first + lane, last);
-        scale_base = uniform((in_a ? p.a_scales : p.b_scales) + (long long)start * p.scale_pitch);
-        scale_offset = (unsigned)((row - start) * p.scale_pitch);
+        scale_base[i] = uniform((in_a ? p.a_scales : p.b_scales) + (long long)start * p.scale_pitch);
+        scale_offset[i] = (unsigned)((row - start) * p.scale_pitch);
     }
 
     const int k_begin = split * p.per_split, k_end = min(p.blocks, k_begin + p.per_split);
-    auto fetch = [&](int k, int buffer) {
+    auto fetch_one = [&](int i, int k, int buffer) {
+        dma16(base[i] + (long long)k * 128, offset[i], lds + (unsigned)(buffer * STEP + (i * NW + wave) * 1024));
+    };
+    auto fetch_scales = [&](int k, int buffer) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-            dma16(base[i] + (long long)k * 128, offset[i], lds + (unsigned)(buffer * STEP + (i * NW + wave) * 1024));
-        if ((k & 3) == 0 || k == k_begin) {  // (a slice may begin inside a word)
-            if (wave < SCALE_LOADS) dma4(scale_base + (k & ~3), scale_offset, lds_scales + (unsigned)(((k >> 2) & 1) * ROWS * 4 + wave * 256));
-        }
+        for (int i = 0; i < SCALE_LOADS; ++i)
+            dma4(scale_base[i] + (k & ~3), scale_offset[i], lds_scales + (unsigned)(buffer * ROWS * 4 + (i * NW + wave) * 256));
     };
 
+    // Two groups of matrix instructions (16 of the contraction each) per chunk of 32.  While a group runs, the next one's
+    // operands are widened between its instructions, and the next chunk's pieces are on their way from LDS.  The barrier
+    // between two steps stands in front of a step's last chunk, whose pieces are in registers by then.
     v16f acc[MI][NI] = {};
+    v4i qa[2][MI], qb[2][NI];
+    v4i fa[2][MI], fb[2][NI];  // bf16
+    float sa[MI], sb[NI];
     const int row_a = wm * WM + (lane & 31), row_b = BM + wn * WN + (lane & 31);
-    if (k_begin < k_end) fetch(k_begin, 0);
-    unsigned word_a[MI], word_b[NI];
-    for (int k = k_begin, buffer = 0; k < k_end; ++k, buffer ^= 1) {
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" : : : "memory");
-        if (k + 1 < k_end) fetch(k + 1, buffer ^ 1);
-        if ((k & 3) == 0 || k == k_begin) {
+    auto read = [&](int to, int buffer, int chunk) {
+        const unsigned char *at = tile + buffer * STEP + ((chunk * 2 + (lane >> 5)) ^ (lane & 7) ^ ((lane >> 3) & 1)) * 16;
 #pragma unroll
-            for (int i = 0; i < MI; ++i) word_a[i] = scale_words[(k >> 2) & 1][row_a + i * 32];
+        for (int i = 0; i < MI; ++i) qa[to][i] = *reinterpret_cast<const v4i *>(at + (row_a + i * 32) * 128);
 #pragma unroll
-            for (int j = 0; j < NI; ++j) word_b[j] = scale_words[(k >> 2) & 1][row_b + j * 32];
-        }
-        float sa[MI], sb[NI];
+        for (int j = 0; j < NI; ++j) qb[to][j] = *reinterpret_cast<const v4i *>(at + (row_b + j * 32) * 128);
+    };
+    auto read_scales = [&](int k, int buffer) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i) sa[i] = scale_factor(word_a[i], k & 3);
+        for (int i = 0; i < MI; ++i) sa[i] = scale_factor(scale_words[buffer][row_a + i * 32], k & 3);
 #pragma unroll
-        for (int j = 0; j < NI; ++j) sb[j] = scale_factor(word_b[j], k & 3);
-        const unsigned char *at = tile + buffer * STEP;
+        for (int j = 0; j < NI; ++j) sb[j] = scale_factor(scale_words[buffer][row_b + j * 32], k & 3);
+    };
+    auto widen_group = [&](int to, int from, int h) {
 #pragma unroll
-        for (int c = 0; c < 8; c += 2) {  // 32 of the contraction: the half waves take a 16-byte piece each
-            const int piece = ((c + (lane >> 5)) ^ (lane & 7)) * 16;
-            v4i qa[MI], qb[NI];
+        for (int j = 0; j < NI; ++j) fb[to][j] = __builtin_bit_cast(v4i, widen(qb[from][j][2 * h], qb[from][j][2 * h + 1], sb[j]));
 #pragma unroll
-            for (int i = 0; i < MI; ++i) qa[i] = *reinterpret_cast<const v4i *>(at + (row_a + i * 32) * 128 + piece);
+        for (int i = 0; i < MI; ++i) fa[to][i] = __builtin_bit_cast(v4i, widen(qa[from][i][2 * h], qa[from][i][2 * h + 1], sa[i]));
+    };
+    // A step's loads go out in four turns in front of as many groups: the last two of step k - 2 (whose buffer they fill)
+    // and the first two of step k - 1, which leaves them four groups, about 2 us, to arrive.
+    constexpr int TURNS = 4;
+    auto fetch_some = [&](int turn, int k, int buffer) {
+        if (turn == 0) fetch_scales(k, buffer);
 #pragma unroll
-            for (int j = 0; j < NI; ++j) qb[j] = *reinterpret_cast<const v4i *>(at + (row_b + j * 32) * 128 + piece);
+        for (int i = 0; i < LOADS; ++i)
+            if (i * TURNS / LOADS == turn) fetch_one(i, k, buffer);
+    };
+    // `after`: how many steps follow, as far as it matters (2 stands for more).
+    auto step = [&](auto after, int k, int buffer) {
+        constexpr int AFTER = decltype(after)::value;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                v8bf va[MI], vb[NI];
-#pragma unroll
-                for (int i = 0; i < MI; ++i) va[i] = widen(qa[i][2 * h], qa[i][2 * h + 1], sa[i]);
-#pragma unroll
-                for (int j = 0; j < NI; ++j) vb[j] = widen(qb[j][2 * h], qb[j][2 * h + 1], sb[j]);
-#pragma unroll
-                for (int i = 0; i < MI; ++i)
-#pragma unroll
-                    for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[i], vb[j], acc[i][j], 0, 0, 0);
+        for (int g = 0; g < 8; ++g) {
+            const int chunk = g >> 1, next = (g + 1) & 1;
+            if ((g & 1) == 0) {
+                if (chunk < 3) {
+                    read((chunk + 1) & 1, buffer, chunk + 1);
+                } else if (AFTER >= 1) {
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+                    read(0, buffer ^ 1, 0);
+                }
             }
+            if (g == 7 && AFTER >= 1) read_scales(k + 1, buffer ^ 1);
+            if (g < 2 && AFTER >= 1) fetch_some(2 + g, k + 1, buffer ^ 1);
+            if (g >= 6 && AFTER >= 2) fetch_some(g - 6, k + 2, buffer);
+            if (g < 7 || AFTER >= 1) widen_group(next, ((g + 1) >> 1) & 1, next);
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, fa[g & 1][i]), __builtin_bit_cast(v8bf, fb[g & 1][j]),
+                                                                         acc[i][j], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < MI * NI; ++t) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                              // a matrix instruction,
+                __builtin_amdgcn_sched_group_barrier(0x002, 4 * (MI + NI) / (MI * NI) + 1, 0);  // its share of the vector ones
+            }
+            // (the widened operands exist here: left to itself the compiler widens them where they are used)
+            if (g < 7 || AFTER >= 1) {
+#pragma unroll
+                for (int i = 0; i < MI; ++i) asm volatile("" : "+v"(fa[next][i]));
+#pragma unroll
+                for (int j = 0; j < NI; ++j) asm volatile("" : "+v"(fb[next][j]));
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
+    };
+    if (k_begin < k_end) {
+#pragma unroll
+        for (int t = 0; t < TURNS; ++t) fetch_some(t, k_begin, 0);
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" : : : "memory");
+        if (k_begin + 1 < k_end) {
+            fetch_some(0, k_begin + 1, 1);
+            fetch_some(1, k_begin + 1, 1);
+        }
+        read(0, 0, 0);
+        read_scales(k_begin, 0);
+        widen_group(0, 0, 0);
+        int k = k_begin, buffer = 0;
+        for (; k + 2 < k_end; ++k, buffer ^= 1) step(std::integral_constant<int, 2>(), k, buffer);
+        if (k + 1 < k_end) {
+            step(std::integral_constant<int, 1>(), k, buffer);
+            ++k;
+            buffer ^= 1;
+        }
+        step(std::integral_constant<int, 0>(), k, buffer);
     }
     float *c = p.c + (long long)split * p.M * p.ldc;
 #pragma unroll
