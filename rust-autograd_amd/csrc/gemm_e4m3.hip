@@ -73,16 +73,17 @@ __device__ inline const unsigned char *uniform(const unsigned char *p)
 // barrier in front of a step's last chunk 101 us, 1.48 ms; one basic block per step (no tests around the loads) and the
 // loads spread over four groups 97 us, 1.44 ms.  Four waves of 128 x 128 need a third less of LDS and widening but stand
 // still together: 99 us, 1.46 ms; loads spread singly between the instructions 100 us, 1.48 ms.
-template <int BM, int BN, int WM, int WN>
+template <int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void gemm_e4m3_tile_kernel(GemmE4m3 p)
 {
     constexpr int WAVES_N = BN / WN, NW = BM / WM * WAVES_N, MI = WM / 32, NI = WN / 32;
     constexpr int ROWS = BM + BN, STEP = ROWS * 128;
     constexpr int LOADS = ROWS / 8 / NW;         // 1 KiB loads (8 rows) of a wave per step
-    constexpr int SCALE_LOADS = ROWS / 64 / NW;  // 64 words of a wave per step
-    static_assert(ROWS % (8 * NW) == 0 && BM % 64 == 0 && BN % 64 == 0 && ROWS % (64 * NW) == 0, "rows divide over the waves");
-    __shared__ __attribute__((aligned(1024))) unsigned char tile[2 * STEP];
-    __shared__ __attribute__((aligned(256))) unsigned scale_words[2][ROWS];
+    constexpr int SCALE_LOADS = (ROWS / 64 + NW - 1) / NW;  // 64 words of a wave per step
+    static_assert(STAGES >= 2 && STAGES <= 4, "ring of two to four steps");
+    static_assert(ROWS % (8 * NW) == 0 && BM % 64 == 0 && BN % 64 == 0, "rows divide over the waves");
+    __shared__ __attribute__((aligned(1024))) unsigned char tile[STAGES * STEP];
+    __shared__ __attribute__((aligned(256))) unsigned scale_words[STAGES][ROWS];
     const unsigned lds = (unsigned)(size_t)(lds_byte_t *)tile, lds_scales = (unsigned)(size_t)(lds_byte_t *)scale_words;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void gemm_e4m3_tile_kerne
     unsigned scale_offset[SCALE_LOADS];
 #pragma unroll
     for (int i = 0; i < SCALE_LOADS; ++i) {
-        const int r0 = (i * NW + wave) * 64;
+        const int r0 = min((i * NW + wave) * 64, ROWS - 64);  // (where they do not divide over the waves, some fetch the last again)
         const bool in_a = r0 < BM;
         const int first = in_a ? m0 + r0 : n0 + r0 - BM, last = (in_a ? p.M : p.N) - 1;
         const int start = min(first, last), row = min(first + lane, last);
@@ -129,7 +130,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void gemm_e4m3_tile_kerne
     auto fetch_scales = [&](int k, int buffer) {
 #pragma unroll
         for (int i = 0; i < SCALE_LOADS; ++i)
-            dma4(scale_base[i] + (k & ~3), scale_offset[i], lds_scales + (unsigned)(buffer * ROWS * 4 + (i * NW + wave) * 256));
+            dma4(scale_base[i] + (k & ~3), scale_offset[i], lds_scales + (unsigned)(buffer * ROWS * 4 + min((i * NW + wave) * 256, ROWS * 4 - 256)));
     };
 
     // Two groups of matrix instructions (16 of the contraction each) per chunk of 32.  While a group runs, the next one's
@@ -159,16 +160,21 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void gemm_e4m3_tile_kerne
 #pragma unroll
         for (int i = 0; i < MI; ++i) fa[to][i] = __builtin_bit_cast(v4i, widen(qa[from][i][2 * h], qa[from][i][2 * h + 1], sa[i]));
     };
-    // A step's loads go out in four turns in front of as many groups: the last two of step k - 2 (whose buffer they fill)
-    // and the first two of step k - 1, which leaves them four groups, about 2 us, to arrive.
-    constexpr int TURNS = 4;
+    // The loads run AHEAD steps in front of the matrix instructions.  A step's go out in four turns in front of as many
+    // groups: the last two of the step whose buffer they fill and the first two of the next.
+    constexpr int TURNS = 4, AHEAD = STAGES - 1;
     auto fetch_some = [&](int turn, int k, int buffer) {
         if (turn == 0) fetch_scales(k, buffer);
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
             if (i * TURNS / LOADS == turn) fetch_one(i, k, buffer);
     };
-    // `after`: how many steps follow, as far as it matters (2 stands for more).
+    auto wrap = [](int buffer) { return buffer >= STAGES ? buffer - STAGES : buffer; };
+    // Waits for the loads of the next step (`later` whole steps have been fetched behind it) and for every wave's reads.
+    auto arrive = [&](auto later) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(decltype(later)::value * (LOADS + SCALE_LOADS)) : "memory");
+    };
+    // `after`: how many steps follow, as far as it matters (AHEAD + 1 stands for more).
     auto step = [&](auto after, int k, int buffer) {
         constexpr int AFTER = decltype(after)::value;
 #pragma unroll
@@ -178,13 +184,13 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void gemm_e4m3_tile_kerne
                 if (chunk < 3) {
                     read((chunk + 1) & 1, buffer, chunk + 1);
                 } else if (AFTER >= 1) {
-                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
-                    read(0, buffer ^ 1, 0);
+                    arrive(std::integral_constant<int, (AFTER < 1 ? 1 : AFTER < AHEAD ? AFTER : AHEAD) - 1>());
+                    read(0, wrap(buffer + 1), 0);
                 }
             }
-            if (g == 7 && AFTER >= 1) read_scales(k + 1, buffer ^ 1);
-            if (g < 2 && AFTER >= 1) fetch_some(2 + g, k + 1, buffer ^ 1);
-            if (g >= 6 && AFTER >= 2) fetch_some(g - 6, k + 2, buffer);
+            if (g == 7 && AFTER >= 1) read_scales(k + 1, wrap(buffer + 1));
+            if (g < 2 && AFTER >= AHEAD) fetch_some(2 + g, k + AHEAD, wrap(buffer + AHEAD));
+            if (g >= 6 && AFTER > AHEAD) fetch_some(g - 6, k + AHEAD + 1, buffer);
             if (g < 7 || AFTER >= 1) widen_group(next, ((g + 1) >> 1) & 1, next);
 #pragma unroll
             for (int i = 0; i < MI; ++i)
@@ -208,24 +214,35 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void gemm_e4m3_tile_kerne
         }
     };
     if (k_begin < k_end) {
+        const int steps = k_end - k_begin;
+        // steps 0 .. AHEAD - 1 whole, and the first two turns of step AHEAD
 #pragma unroll
-        for (int t = 0; t < TURNS; ++t) fetch_some(t, k_begin, 0);
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" : : : "memory");
-        if (k_begin + 1 < k_end) {
-            fetch_some(0, k_begin + 1, 1);
-            fetch_some(1, k_begin + 1, 1);
+        for (int a = 0; a < AHEAD; ++a)
+            if (a < steps)
+#pragma unroll
+                for (int t = 0; t < TURNS; ++t) fetch_some(t, k_begin + a, a);
+        if (steps >= AHEAD) arrive(std::integral_constant<int, AHEAD - 1>());
+        else arrive(std::integral_constant<int, 0>());
+        if (AHEAD < steps) {
+            fetch_some(0, k_begin + AHEAD, AHEAD);
+            fetch_some(1, k_begin + AHEAD, AHEAD);
         }
         read(0, 0, 0);
         read_scales(k_begin, 0);
         widen_group(0, 0, 0);
         int k = k_begin, buffer = 0;
-        for (; k + 2 < k_end; ++k, buffer ^= 1) step(std::integral_constant<int, 2>(), k, buffer);
-        if (k + 1 < k_end) {
-            step(std::integral_constant<int, 1>(), k, buffer);
-            ++k;
-            buffer ^= 1;
-        }
-        step(std::integral_constant<int, 0>(), k, buffer);
+        for (; k + AHEAD + 1 < k_end; ++k, buffer = wrap(buffer + 1)) step(std::integral_constant<int, AHEAD + 1>(), k, buffer);
+        auto last = [&](auto after) {
+            if (k_end - 1 - k == decltype(after)::value) {
+                step(after, k, buffer);
+                ++k;
+                buffer = wrap(buffer + 1);
+            }
+        };
+        if constexpr (AHEAD >= 3) last(std::integral_constant<int, 3>());
+        if constexpr (AHEAD >= 2) last(std::integral_constant<int, 2>());
+        last(std::integral_constant<int, 1>());
+        last(std::integral_constant<int, 0>());
     }
     float *c = p.c + (long long)split * p.M * p.ldc;
 #pragma unroll
@@ -264,79 +281,109 @@ __global__ __launch_bounds__(256) void gemm_e4m3_fold_kernel(const float *__rest
 // ---- few rows ---------------------------------------------------------------------------------------------------------
 // Up to 16 * MT rows of A against 16 rows of B per block, operands straight from global memory into the matrix unit's
 // layout: the weight is read once, in whole 512-byte pieces of its rows, and nothing is shared between waves but the
-// sums.  The waves take pieces of 512 of the contraction in turn; their sums are added in order through LDS.
-// Lane l holds row l % 16 and 32 consecutive bytes of each 128: group l / 16 of four.
-// FROM_F32: A is x itself, rounded on the way as ag_quantize_e4m3_f32 rounds it.
-constexpr int kSkinnyRows = 64;
+// sums.  The waves take pieces of 512 of the contraction in turn, with every load of a piece in flight at once; their sums
+// are added in order through LDS.  Lane l holds row l % 16 and 32 consecutive bytes of each 128: group l / 16 of four.
+// XR > 0: A is x itself, at most XR rows of it, rounded on the way as ag_quantize_e4m3_f32 rounds it: a wave rounds its
+// pieces of the rows with 32 lanes to a block and hands the bytes to the lanes that multiply them through LDS.  One row
+// against 4096 x 4096 takes 7.1 us that way (2.4 TB/s of weight: launch, one round of loads, the sums), against 16384 x
+// 4096 17.7 us (3.8 TB/s); as two launches 10.2 and 20.8 us, and with the rows rounded by the 4 lanes of the matrix
+// layout that hold them 12.0 and 32 us.  At 4 rows the two ways are even (10.0 and 10.2, 22.8 and 20.8 us).
+constexpr int kRoundedRows = 4;
 
-template <int MT, int NW, bool FROM_F32>
+template <int MT, int NW, int XR>
 __global__ __launch_bounds__(NW * 64) void gemm_e4m3_skinny_kernel(GemmE4m3 p, const float *__restrict__ x, long long ldx, int K)
 {
-    static_assert(!FROM_F32 || MT == 1, "rounded in place for few rows only");
+    static_assert(XR == 0 || (MT == 1 && XR == 4), "rounded on the way for few rows only");
+    constexpr int PIECE = 512 + 16;  // bytes of a row's piece in LDS: 16 more than it has, so that rows fall on other banks
     __shared__ float sums[NW][MT][256];
+    __shared__ __attribute__((aligned(16))) unsigned char rounded[XR > 0 ? NW : 1][XR > 0 ? XR : 1][PIECE];
+    __shared__ __attribute__((aligned(4))) unsigned char rounded_scales[XR > 0 ? NW : 1][XR > 0 ? XR : 1][4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, group = lane >> 4;
     const int n0 = blockIdx.x * 16;
-    const int row_b = min(n0 + r16, p.N - 1);
-    const unsigned char *b = p.b + row_b * p.pitch + group * 32, *b_scales = p.b_scales + (long long)row_b * p.scale_pitch;
     const int words = (p.blocks + 3) / 4;
+    const int row_b = min(n0 + r16, p.N - 1);
     v4f acc[MT] = {};
     for (int w = wave; w < words; w += NW) {
         const int count = min(4, p.blocks - w * 4);
-        v4i qb[4][2];
-        const unsigned word_b = *reinterpret_cast<const unsigned *>(b_scales + w * 4);
+        v4i qb[4][2], qa[MT][4][2];
+        unsigned word_a[MT];
+        const unsigned char *b = p.b + row_b * p.pitch + (long long)w * 512 + group * 32, *a[MT];
+        const unsigned word_b = *reinterpret_cast<const unsigned *>(p.b_scales + (long long)row_b * p.scale_pitch + w * 4);
+        if (XR == 0)
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (u < count)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) qb[u][h] = *reinterpret_cast<const v4i *>(b + (long long)(w * 4 + u) * 128 + h * 16);
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            v4i qa[4][2];
-            unsigned word_a = 0;
-            if (FROM_F32) {
-                const bool here = r16 < p.M;
-                const float *row = x + (here ? r16 : 0) * ldx;
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (u < count) {
-                        quad_t v[8];
-                        unsigned top = 0;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            v[i] = here ? load_quad(row, (long long)(w * 4 + u) * 128 + group * 32 + i * 4, K) : quad_t{0.f, 0.f, 0.f, 0.f};
-                            top = max(top, finite_magnitude(v[i]));
-                        }
-                        top = max(top, (unsigned)__shfl_xor((int)top, 16, 64));
-                        top = max(top, (unsigned)__shfl_xor((int)top, 32, 64));
-                        const unsigned sb = scale_byte(top);
-                        const float inv = scale_inverse(sb);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) qa[u][i / 4][i % 4] = (int)round_e4m3(v[i], inv);
-                        word_a |= sb << (8 * u);
-                    }
-            } else {
+            for (int t = 0; t < MT; ++t) {
                 const int row_a = min(t * 16 + r16, p.M - 1);
-                word_a = *reinterpret_cast<const unsigned *>(p.a_scales + (long long)row_a * p.scale_pitch + w * 4);
-                const unsigned char *a = p.a + row_a * p.pitch + group * 32;
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (u < count)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) qa[u][h] = *reinterpret_cast<const v4i *>(a + (long long)(w * 4 + u) * 128 + h * 16);
+                a[t] = p.a + row_a * p.pitch + (long long)w * 512 + group * 32;
+                word_a[t] = *reinterpret_cast<const unsigned *>(p.a_scales + (long long)row_a * p.scale_pitch + w * 4);
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (u < count) {
-                    const float sa = scale_factor(word_a, u), sb = scale_factor(word_b, u);
+        for (int u = 0; u < 4; ++u) {  // (in the order of their use: they arrive in it)
+            const int at = min(u, count - 1) * 128;  // (a piece that ends early reads its last block again)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h) {
+                qb[u][h] = *reinterpret_cast<const v4i *>(b + at + h * 16);
+                if (XR == 0)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(qa[u][h][2 * e], qa[u][h][2 * e + 1], sa),
-                                                                            widen(qb[u][h][2 * e], qb[u][h][2 * e + 1], sb), acc[t], 0, 0, 0);
-                }
+                    for (int t = 0; t < MT; ++t) qa[t][u][h] = *reinterpret_cast<const v4i *>(a[t] + at + h * 16);
+            }
         }
+        if (XR > 0) {
+            const int half = lane >> 5, l31 = lane & 31;
+            auto round_rows = [&](auto several) {  // the first rows of x (the last one again where there are fewer), loaded together
+                constexpr int ROWS = decltype(several)::value;
+                quad_t v[ROWS][2];  // blocks half and half + 2 of the piece
+                const long long k0 = (long long)w * 512 + half * 128 + l31 * 4;
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) {
+                    const float *row = x + min(r, p.M - 1) * ldx;
+                    if ((long long)(w + 1) * 512 <= K) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) v[r][i] = *reinterpret_cast<const quad_any_t *>(row + k0 + i * 256);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) v[r][i] = load_quad(row, k0 + i * 256, K);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const unsigned sb = scale_byte(half_wave_max(finite_magnitude(v[r][i])));
+                        *reinterpret_cast<unsigned *>(&rounded[wave][r][(half + 2 * i) * 128 + l31 * 4]) = round_e4m3(v[r][i], scale_inverse(sb));
+                        if (l31 == 0) rounded_scales[wave][r][half + 2 * i] = (unsigned char)sb;
+                    }
+            };
+            if (p.M == 1) round_rows(std::integral_constant<int, 1>());
+            else if (p.M == 2) round_rows(std::integral_constant<int, 2>());
+            else round_rows(std::integral_constant<int, 4>());
+            __builtin_amdgcn_wave_barrier();  // (only this wave reads them: its LDS accesses complete in order)
+            const bool here = r16 < p.M;
+            word_a[0] = here ? *reinterpret_cast<const unsigned *>(rounded_scales[wave][here ? r16 : 0]) : 0x7f7f7f7fu;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const v4i q = *reinterpret_cast<const v4i *>(&rounded[wave][here ? r16 : 0][u * 128 + group * 32 + h * 16]);
+                    qa[0][u][h] = here ? q : v4i{0, 0, 0, 0};
+                }
+            __builtin_amdgcn_wave_barrier();
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (u < count) {
+                const float sb = scale_factor(word_b, u);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const v8bf vb = widen(qb[u][h][2 * e], qb[u][h][2 * e + 1], sb);
+#pragma unroll
+                        for (int t = 0; t < MT; ++t)
+                            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(qa[t][u][h][2 * e], qa[t][u][h][2 * e + 1], scale_factor(word_a[t], u)), vb,
+                                                                            acc[t], 0, 0, 0);
+                    }
+            }
     }
     // lane l holds column l % 16 and rows 4 (l / 16) .. + 3
 #pragma unroll
@@ -358,27 +405,38 @@ __global__ __launch_bounds__(NW * 64) void gemm_e4m3_skinny_kernel(GemmE4m3 p, c
 ag_status_t quantize_e4m3(const char *who, hipStream_t st, const float *x, long long ldx, int rows, int cols, unsigned char *q, unsigned char *scales,
                           unsigned char *qt, unsigned char *scales_t);
 
+// Tiles of the output (0: the kernel for few rows) and slices of the contraction, by the extents alone.  Times in us:
+//   up to 16 rows               the kernel for few rows: 8 rows x 16384 x 4096 18.0, with tiles of 64 21.4;
+//   up to 32 rows, at most a block per CU with a piece per wave      32 x 4096 x 4096 9.3, with tiles of 64 11.3 (but 32 x
+//                               16384 x 4096 32.8 against 21.4, and 40 x 300 x 8192 18.0 against 10.7);
+//   at most two tiles of 64 per CU       these, four steps deep, the contraction cut until there is a block per CU, not below
+//                               8 steps to a slice: 64 x 1000 x 8192 11.6 in 8 slices, 13.6 in 4 (tiles of 128, 12 slices: 15.7);
+//                               256 x 4096 x 4096 19.7 (tiles of 128 22.6); 64 x 8192 x 1024 7.6, in 2 slices 10.1;
+//   at most a tile of 128 per CU         these, four steps deep: 1024 x 4096 x 4096 36.0 (two steps deep 44.8);
+//   else tiles of 128, two blocks per CU, or of 256, one per CU, whichever needs less time by whole rounds of blocks, a round
+//                               of the smaller taking 0.62 of one of the larger (2048 x 4096 x 4096: 62 and 72; 4096^3: 128 and 97).
 struct Plan {
-    int bm, bn, splits;
+    int tile, splits;
+    bool deep;
 };
 
 static Plan plan_product(int M, int N, int K)
 {
-    const long long blocks = (long long)(e4m3_pitch(K) / kE4m3Block), cus = device_cus();
-    auto tiles = [&](int t) { return (long long)((M + t - 1) / t) * ((N + t - 1) / t); };
-    Plan f = {256, 256, 1};
-    if (tiles(256) < cus * 3 / 4) {
-        f = {128, 128, 1};
-        const long long want = (2 * cus) / (tiles(128) ? tiles(128) : 1);
-        f.splits = (int)(want < 1 ? 1 : want > 16 ? 16 : want);
-        while (f.splits > 1 && blocks / f.splits < 4) --f.splits;
+    const long long steps = (long long)(e4m3_pitch(K) / kE4m3Block), cus = device_cus();
+    auto tiles = [&](long long t) { return (M + t - 1) / t * ((N + t - 1) / t); };
+    if (M <= 16 || (M <= 32 && N <= 16 * cus && steps <= 32)) return {0, 1, false};
+    if (tiles(64) <= 2 * cus) {
+        const long long fill = cus / tiles(64), deep = steps / 8;
+        return {64, (int)(fill < deep ? (fill > 1 ? fill : 1) : (deep > 1 ? deep : 1)), true};
     }
-    return f;
+    if (tiles(128) <= cus) return {128, 1, true};
+    const long long rounds128 = (tiles(128) + 2 * cus - 1) / (2 * cus), rounds256 = (tiles(256) + cus - 1) / cus;
+    return {rounds128 * 62 < rounds256 * 100 ? 128 : 256, 1, false};
 }
 
 static size_t product_workspace(int M, int N, int K)
 {
-    if (M <= 0 || N <= 0 || K <= 0 || M <= kSkinnyRows) return 0;
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
     const Plan f = plan_product(M, N, K);
     return f.splits > 1 ? (size_t)f.splits * M * N * sizeof(float) : 0;
 }
@@ -395,31 +453,29 @@ static ag_status_t check_product(const char *who, int M, int N, int K, int ldc, 
     return AG_OK;
 }
 
-template <int MT, bool FROM_F32>
+template <int MT, int XR>
 static void launch_skinny(hipStream_t st, const GemmE4m3 &p, const float *x, long long ldx, int K)
 {
     const dim3 grid((unsigned)((p.N + 15) / 16));
-    const int words = (p.blocks + 3) / 4;
+    const int words = (p.blocks + 3) / 4;  // a wave each, up to eight
     if (words <= 2)
-        hipLaunchKernelGGL((gemm_e4m3_skinny_kernel<MT, 2, FROM_F32>), grid, dim3(128), 0, st, p, x, ldx, K);
+        hipLaunchKernelGGL((gemm_e4m3_skinny_kernel<MT, 2, XR>), grid, dim3(128), 0, st, p, x, ldx, K);
     else if (words <= 4)
-        hipLaunchKernelGGL((gemm_e4m3_skinny_kernel<MT, 4, FROM_F32>), grid, dim3(256), 0, st, p, x, ldx, K);
+        hipLaunchKernelGGL((gemm_e4m3_skinny_kernel<MT, 4, XR>), grid, dim3(256), 0, st, p, x, ldx, K);
     else
-        hipLaunchKernelGGL((gemm_e4m3_skinny_kernel<MT, 8, FROM_F32>), grid, dim3(512), 0, st, p, x, ldx, K);
+        hipLaunchKernelGGL((gemm_e4m3_skinny_kernel<MT, 8, XR>), grid, dim3(512), 0, st, p, x, ldx, K);
 }
 
 static ag_status_t product(const char *who, hipStream_t st, GemmE4m3 p, int K, void *ws)
 {
-    if (p.M <= kSkinnyRows) {
-        if (p.M <= 16) launch_skinny<1, false>(st, p, nullptr, 0, K);
-        else if (p.M <= 32) launch_skinny<2, false>(st, p, nullptr, 0, K);
-        else if (p.M <= 48) launch_skinny<3, false>(st, p, nullptr, 0, K);
-        else launch_skinny<4, false>(st, p, nullptr, 0, K);
+    const Plan f = plan_product(p.M, p.N, K);
+    if (f.tile == 0) {
+        if (p.M <= 16) launch_skinny<1, 0>(st, p, nullptr, 0, K);
+        else launch_skinny<2, 0>(st, p, nullptr, 0, K);
         return check_launch(who);
     }
-    const Plan f = plan_product(p.M, p.N, K);
-    p.tiles_m = (p.M + f.bm - 1) / f.bm;
-    p.tiles_n = (p.N + f.bn - 1) / f.bn;
+    p.tiles_m = (p.M + f.tile - 1) / f.tile;
+    p.tiles_n = (p.N + f.tile - 1) / f.tile;
     p.splits = f.splits;
     p.per_split = (p.blocks + f.splits - 1) / f.splits;
     const unsigned long long grid = (unsigned long long)p.tiles_m * p.tiles_n * f.splits;
@@ -427,10 +483,14 @@ static ag_status_t product(const char *who, hipStream_t st, GemmE4m3 p, int K, v
     float *c = p.c;
     const long long ldc = p.ldc;
     if (f.splits > 1) p.c = static_cast<float *>(ws), p.ldc = p.N;
-    if (f.bm == 256)
-        hipLaunchKernelGGL((gemm_e4m3_tile_kernel<256, 256, 128, 64>), dim3((unsigned)grid), dim3(512), 0, st, p);
+    if (f.tile == 256)
+        hipLaunchKernelGGL((gemm_e4m3_tile_kernel<256, 256, 128, 64, 2>), dim3((unsigned)grid), dim3(512), 0, st, p);
+    else if (f.tile == 128 && f.deep)
+        hipLaunchKernelGGL((gemm_e4m3_tile_kernel<128, 128, 64, 64, 4>), dim3((unsigned)grid), dim3(256), 0, st, p);
+    else if (f.tile == 128)
+        hipLaunchKernelGGL((gemm_e4m3_tile_kernel<128, 128, 64, 64, 2>), dim3((unsigned)grid), dim3(256), 0, st, p);
     else
-        hipLaunchKernelGGL((gemm_e4m3_tile_kernel<128, 128, 64, 64>), dim3((unsigned)grid), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((gemm_e4m3_tile_kernel<64, 64, 32, 32, 4>), dim3((unsigned)grid), dim3(256), 0, st, p);
     if (f.splits > 1) {
         const long long cells = (long long)p.M * p.N;
         hipLaunchKernelGGL(gemm_e4m3_fold_kernel, dim3((unsigned)((cells + 1023) / 1024)), dim3(256), 0, st, static_cast<const float *>(ws), c, ldc, p.M,
@@ -450,7 +510,7 @@ static GemmE4m3 params(int M, int N, int K, const unsigned char *a, const unsign
 static size_t rounded_bytes(int M, int K) { return (size_t)M * e4m3_pitch(K) + ((size_t)M * e4m3_scale_pitch(K) + 15) / 16 * 16; }
 
 // Few enough rows of x that each block rounds them for itself.
-static bool rounds_in_place(int M) { return M <= 4; }
+static bool rounds_in_place(int M) { return M <= kRoundedRows; }
 
 }  // namespace ag
 
@@ -492,7 +552,7 @@ extern "C" ag_status_t ag_quantize_matmul_e4m3_f32(ag_stream_t stream, int M, in
     AG_REQUIRE(need == 0 || aligned16(ws), AG_ERR_INVALID_DIMS, "quantize_matmul_e4m3: misaligned workspace");
     hipStream_t st = as_stream(stream);
     if (rounds_in_place(M)) {
-        launch_skinny<1, true>(st, params(M, N, K, nullptr, nullptr, B, b_scales, C, ldc), x, ldx, K);
+        launch_skinny<1, kRoundedRows>(st, params(M, N, K, nullptr, nullptr, B, b_scales, C, ldc), x, ldx, K);
         return check_launch("quantize_matmul_e4m3");
     }
     unsigned char *q = static_cast<unsigned char *>(ws), *scales = q + (size_t)M * e4m3_pitch(K);
