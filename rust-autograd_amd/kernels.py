@@ -18,7 +18,8 @@ def _ptr(t):
 
 
 def _stream():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # (the handle itself: making a Stream object of it costs ten times as much as looking it up)
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _f32(t, name):
@@ -522,6 +523,8 @@ def sparse_softmax_cross_entropy_grad_from_logits(logits, labels, gy):
 
 
 # ------------------------------------------------------------------------------------------ 8-bit operands
+# The launchers from here on serve calls that take a few microseconds on the device, so what they do on the host counts:
+# pointers travel as plain integers, and each tensor is looked at once.
 class E4m3(NamedTuple):
     """An 8-bit operand: q [rows, pitch(n)] of float8_e4m3fn, scales [rows, scale_pitch(n)] of float8_e8m0fnu (one power of
     two per block of 128), n elements per row along the contraction; an element is q * scale."""
@@ -539,50 +542,47 @@ class E4m3(NamedTuple):
         return (self.q.float().view(self.q.shape[0], -1, 128) * power[:, :, None]).view(self.q.shape)[:, : self.n]
 
 
-def _e4m3_empty(rows, n, like):
-    L = capi.lib()
-    return E4m3(_empty((rows, L.ag_e4m3_pitch(n)), like, torch.float8_e4m3fn),
-                _empty((rows, L.ag_e4m3_scale_pitch(n)), like, torch.float8_e8m0fnu), n)
-
-
-def _e4m3(e, name):
-    """Checks an 8-bit operand against the layout that the kernels read."""
-    if not (isinstance(e, E4m3) and e.q.is_cuda and e.scales.is_cuda):
-        raise capi.TypeUnsupported(f"{name}: expected an E4m3 of CUDA tensors")
-    if e.q.dtype != torch.float8_e4m3fn or e.scales.dtype != torch.float8_e8m0fnu:
-        raise capi.TypeUnsupported(f"{name}: expected float8_e4m3fn values and float8_e8m0fnu scales")
-    rows, pitch = e.q.shape
-    if pitch != -(-e.n // 128) * 128 or e.scales.shape != (rows, -(-e.n // 512) * 4):
-        raise capi.IncompatibleShape(f"{name}: values {list(e.q.shape)} and scales {list(e.scales.shape)} are not those of "
-                                     f"rows of {e.n} elements")
-    _on_current_device(name, e.q, e.scales)
-    return E4m3(e.q.contiguous(), e.scales.contiguous(), e.n)
-
-
-def _on_current_device(name, *tensors):
-    """A launch goes to the current device's stream: tensors of another device are refused."""
-    at = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.device.index != at:
-            raise capi.TypeUnsupported(f"{name}: a tensor on {t.device} while cuda:{at} is the current device")
+def _here(t, name, dtype=torch.float32):
+    """t, contiguous, if it is a tensor of that type on the current device (a launch goes to that device's stream)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise capi.TypeUnsupported(f"{name}: expected a CUDA tensor")
+    if t.dtype is not dtype:
+        raise capi.TypeUnsupported(f"{name}: expected {dtype} (got {t.dtype})")
+    if t.get_device() != torch._C._cuda_getDevice():
+        raise capi.TypeUnsupported(f"{name}: a tensor on {t.device} while cuda:{torch.cuda.current_device()} is the current device")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _matrix(x, name):
-    x = _f32(x, name)
-    _on_current_device(name, x)
+    x = _here(x, name)
     if x.dim() != 2:
         raise capi.IncompatibleShape(f"{name}: input must be 2D (got {list(x.shape)})")
     return x
+
+
+def _e4m3_empty(rows, n, device):
+    return E4m3(torch.empty((rows, -(-n // 128) * 128), dtype=torch.float8_e4m3fn, device=device),
+                torch.empty((rows, -(-n // 512) * 4), dtype=torch.float8_e8m0fnu, device=device), n)
+
+
+def _e4m3(e, name):
+    """Checks an 8-bit operand against the layout that the kernels read: (values, scales, rows, n)."""
+    if not isinstance(e, E4m3):
+        raise capi.TypeUnsupported(f"{name}: expected an E4m3 of CUDA tensors")
+    q, scales = _here(e.q, name, torch.float8_e4m3fn), _here(e.scales, name, torch.float8_e8m0fnu)
+    if q.dim() != 2 or q.shape[1] != -(-e.n // 128) * 128 or scales.shape != (q.shape[0], -(-e.n // 512) * 4):
+        raise capi.IncompatibleShape(f"{name}: values {list(q.shape)} and scales {list(scales.shape)} are not those of rows of {e.n} elements")
+    return q, scales, q.shape[0], e.n
 
 
 def quantize_e4m3(x, transpose=False):
     """x [rows, cols] rounded to 8 bits along its rows; transpose=True: along its columns, as the transposed array."""
     x = _matrix(x, "quantize_e4m3")
     rows, cols = x.shape
-    e = _e4m3_empty(cols, rows, x) if transpose else _e4m3_empty(rows, cols, x)
-    q, s = _ptr(e.q), _ptr(e.scales)
-    check(capi.lib().ag_quantize_e4m3_f32(_stream(), _ptr(x), cols, rows, cols, None if transpose else q, None if transpose else s,
-                                          q if transpose else None, s if transpose else None))
+    e = _e4m3_empty(cols, rows, x.device) if transpose else _e4m3_empty(rows, cols, x.device)
+    q, s = e.q.data_ptr(), e.scales.data_ptr()
+    out = (None, None, q, s) if transpose else (q, s, None, None)
+    check(capi.lib().ag_quantize_e4m3_f32(_stream(), x.data_ptr(), cols, rows, cols, *out))
     return e
 
 
@@ -590,8 +590,9 @@ def quantize_e4m3_both(x):
     """Both of quantize_e4m3's results from one pass over x: (along rows, transposed)."""
     x = _matrix(x, "quantize_e4m3")
     rows, cols = x.shape
-    e, t = _e4m3_empty(rows, cols, x), _e4m3_empty(cols, rows, x)
-    check(capi.lib().ag_quantize_e4m3_f32(_stream(), _ptr(x), cols, rows, cols, _ptr(e.q), _ptr(e.scales), _ptr(t.q), _ptr(t.scales)))
+    e, t = _e4m3_empty(rows, cols, x.device), _e4m3_empty(cols, rows, x.device)
+    check(capi.lib().ag_quantize_e4m3_f32(_stream(), x.data_ptr(), cols, rows, cols, e.q.data_ptr(), e.scales.data_ptr(), t.q.data_ptr(),
+                                          t.scales.data_ptr()))
     return e, t
 
 
@@ -599,144 +600,149 @@ def matmul_e4m3(a, b):
     """a . b^T of two 8-bit operands, in f32.  For y = x . w (x [M,K], w [K,N]): matmul_e4m3(quantize_e4m3(x),
     quantize_e4m3(w, transpose=True)); its gradients are matmul_e4m3(quantize_e4m3(gy), quantize_e4m3(w)) and
     matmul_e4m3(quantize_e4m3(x, transpose=True), quantize_e4m3(gy, transpose=True))."""
-    a, b = _e4m3(a, "matmul_e4m3"), _e4m3(b, "matmul_e4m3")
-    if a.n != b.n:
-        raise capi.IncompatibleShape(f"matmul_e4m3: contractions of {a.n} and {b.n} elements")
-    m, n, k = a.rows, b.rows, a.n
-    c = _empty((m, n), a.q)
+    qa, sa, m, k = _e4m3(a, "matmul_e4m3")
+    qb, sb, n, kb = _e4m3(b, "matmul_e4m3")
+    if k != kb:
+        raise capi.IncompatibleShape(f"matmul_e4m3: contractions of {k} and {kb} elements")
+    c = torch.empty((m, n), dtype=torch.float32, device=qa.device)
     L = capi.lib()
     nbytes = L.ag_matmul_e4m3_f32_workspace(m, n, k)
     ws = _ws(nbytes, c) if nbytes else None
-    check(L.ag_matmul_e4m3_f32(_stream(), m, n, k, _ptr(a.q), _ptr(a.scales), _ptr(b.q), _ptr(b.scales), _ptr(c), n, _ptr(ws), nbytes))
+    check(L.ag_matmul_e4m3_f32(_stream(), m, n, k, qa.data_ptr(), sa.data_ptr(), qb.data_ptr(), sb.data_ptr(), c.data_ptr(), n,
+                               ws.data_ptr() if nbytes else None, nbytes))
     return c
 
 
 def quantize_matmul_e4m3(x, b):
     """quantize_e4m3(x) . b^T in one call: a layer whose weight was laid out in 8 bits once."""
-    x, b = _matrix(x, "quantize_matmul_e4m3"), _e4m3(b, "quantize_matmul_e4m3")
+    x = _matrix(x, "quantize_matmul_e4m3")
+    q, s, n, kb = _e4m3(b, "quantize_matmul_e4m3")
     m, k = x.shape
-    if k != b.n:
-        raise capi.IncompatibleShape(f"quantize_matmul_e4m3: contractions of {k} and {b.n} elements")
-    n = b.rows
-    c = _empty((m, n), x)
+    if k != kb:
+        raise capi.IncompatibleShape(f"quantize_matmul_e4m3: contractions of {k} and {kb} elements")
+    c = torch.empty((m, n), dtype=torch.float32, device=x.device)
     L = capi.lib()
     nbytes = L.ag_quantize_matmul_e4m3_f32_workspace(m, n, k)
     ws = _ws(nbytes, x) if nbytes else None
-    check(L.ag_quantize_matmul_e4m3_f32(_stream(), m, n, k, _ptr(x), k, _ptr(b.q), _ptr(b.scales), _ptr(c), n, _ptr(ws), nbytes))
+    check(L.ag_quantize_matmul_e4m3_f32(_stream(), m, n, k, x.data_ptr(), k, q.data_ptr(), s.data_ptr(), c.data_ptr(), n,
+                                        ws.data_ptr() if nbytes else None, nbytes))
     return c
 
 
 # ------------------------------------------------------------------------------------------ RMS norm
-def _rms_norm(x, weight, eps, residual, want_y, want_e4m3):
-    x, weight = _f32(x, "rms_norm"), _f32(weight, "rms_norm")
+def _rms_norm(x, weight, eps, residual, e4m3):
+    x, weight = _here(x, "rms_norm"), _here(weight, "rms_norm")
     if x.dim() < 1 or weight.dim() != 1 or weight.shape[0] != x.shape[-1]:
         raise capi.IncompatibleShape(f"rms_norm: weight {list(weight.shape)} for rows of {list(x.shape)}")
-    h = x
+    h, res = x, None
     if residual is not None:
-        residual = _f32(residual, "rms_norm")
-        if residual.shape != x.shape:
-            raise capi.IncompatibleShape(f"rms_norm: residual {list(residual.shape)} and input {list(x.shape)}")
+        res = _here(residual, "rms_norm")
+        if res.shape != x.shape:
+            raise capi.IncompatibleShape(f"rms_norm: residual {list(res.shape)} and input {list(x.shape)}")
         h = torch.empty_like(x)
-    _on_current_device("rms_norm", x, weight, residual)
     n = x.shape[-1]
     rows = x.numel() // n if n else 0
-    y = torch.empty_like(x) if want_y else None
-    e = _e4m3_empty(rows, n, x) if want_e4m3 else None
-    rstd = _empty((rows,), x)
-    check(capi.lib().ag_rms_norm_f32(_stream(), _ptr(x), _ptr(residual), _ptr(weight), eps, None if residual is None else _ptr(h), _ptr(y),
-                                     _ptr(e.q) if e else None, _ptr(e.scales) if e else None, _ptr(rstd), rows, n))
-    return y, e, h, rstd
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+    if e4m3:
+        y = _e4m3_empty(rows, n, x.device)
+        out = (None, y.q.data_ptr(), y.scales.data_ptr())
+    else:
+        y = torch.empty_like(x)
+        out = (y.data_ptr(), None, None)
+    check(capi.lib().ag_rms_norm_f32(_stream(), x.data_ptr(), res.data_ptr() if res is not None else None, weight.data_ptr(), eps,
+                                     h.data_ptr() if res is not None else None, *out, rstd.data_ptr(), rows, n))
+    return y, h, rstd
 
 
 def rms_norm(x, weight, eps=1e-6, residual=None):
     """(y, h, rstd): h = x + residual (x itself without one), y = h / sqrt(mean(h^2) + eps) * weight over the last axis."""
-    y, _, h, rstd = _rms_norm(x, weight, eps, residual, True, False)
-    return y, h, rstd
+    return _rms_norm(x, weight, eps, residual, False)
 
 
 def rms_norm_e4m3(x, weight, eps=1e-6, residual=None):
     """(e, h, rstd): rms_norm whose y leaves as an 8-bit operand, the bits of quantize_e4m3(y); the rows are those of x
     viewed as a matrix."""
-    _, e, h, rstd = _rms_norm(x, weight, eps, residual, False, True)
-    return e, h, rstd
+    return _rms_norm(x, weight, eps, residual, True)
 
 
 def rms_norm_grad(h, weight, rstd, gy, gh=None):
     """(gx, gw) from rms_norm's h and rstd; gh: the gradient that reaches h on other ways, added to gx."""
-    h, weight, rstd, gy = (_f32(t, "rms_norm_grad") for t in (h, weight, rstd, gy))
+    h, weight, rstd, gy = (_here(t, "rms_norm_grad") for t in (h, weight, rstd, gy))
     n = h.shape[-1] if h.dim() else 0
     rows = h.numel() // n if n else 0
     if weight.shape != (n,) or rstd.shape != (rows,) or gy.shape != h.shape:
         raise capi.IncompatibleShape(f"rms_norm_grad: h {list(h.shape)}, weight {list(weight.shape)}, rstd {list(rstd.shape)}, "
                                      f"gy {list(gy.shape)}")
     if gh is not None:
-        gh = _f32(gh, "rms_norm_grad")
+        gh = _here(gh, "rms_norm_grad")
         if gh.shape != h.shape:
             raise capi.IncompatibleShape(f"rms_norm_grad: gh {list(gh.shape)} and h {list(h.shape)}")
-    _on_current_device("rms_norm_grad", h, weight, rstd, gy, gh)
     gx, gw = torch.empty_like(h), torch.empty_like(weight)
     L = capi.lib()
     ws = _ws(L.ag_rms_norm_grad_f32_workspace(rows, n), h)
-    check(L.ag_rms_norm_grad_f32(_stream(), _ptr(h), _ptr(weight), _ptr(rstd), _ptr(gy), _ptr(gh), _ptr(gx), _ptr(gw), rows, n, _ptr(ws),
-                                 ws.numel()))
+    check(L.ag_rms_norm_grad_f32(_stream(), h.data_ptr(), weight.data_ptr(), rstd.data_ptr(), gy.data_ptr(), None if gh is None else gh.data_ptr(),
+                                 gx.data_ptr(), gw.data_ptr(), rows, n, ws.data_ptr(), ws.numel()))
     return gx, gw
 
 
 # ------------------------------------------------------------------------------------------ clipping
-def _arrays(xs, name):
-    """Dense f32 CUDA tensors as host tables: (pointers, element counts, count)."""
-    n = len(xs)
+def _sizes(xs, name):
+    """Element counts of dense f32 tensors of the current device."""
+    here, f32, ns = torch._C._cuda_getDevice() if len(xs) else 0, torch.float32, []
     for t in xs:
-        if not (t.is_cuda and t.dtype == torch.float32):
-            raise capi.TypeUnsupported(f"{name}: only f32 CUDA tensors are supported")
+        if t.dtype is not f32 or t.get_device() != here:
+            raise capi.TypeUnsupported(f"{name}: only f32 tensors of the current CUDA device are supported")
         if not t.is_contiguous():
             raise capi.IncompatibleShape(f"{name}: tensors must be contiguous")
-    _on_current_device(name, *xs)
-    return (C.c_void_p * max(n, 1))(*[t.data_ptr() for t in xs]), (C.c_size_t * max(n, 1))(*[t.numel() for t in xs]), n
+        ns.append(t.numel())
+    return ns
 
 
-def _clip(xs):
-    return _empty((2,), xs[0]) if len(xs) else torch.empty(2, dtype=torch.float32, device="cuda")
+def _pointers(xs):
+    return (C.c_void_p * max(len(xs), 1))(*[t.data_ptr() for t in xs])
+
+
+def _norm_call(xs, ns):
+    """Host tables, result and workspace of a norm over the tensors."""
+    table = (C.c_size_t * max(len(ns), 1))(*ns)
+    clip = torch.empty(2, dtype=torch.float32, device=xs[0].device if len(xs) else "cuda")
+    return table, clip, _ws(capi.lib().ag_global_norm_f32_workspace(len(ns), table), clip)
+
+
+def _global_norm(xs, ns, max_norm):
+    table, clip, ws = _norm_call(xs, ns)
+    check(capi.lib().ag_global_norm_f32(_stream(), len(ns), _pointers(xs), table, max_norm, clip.data_ptr(), ws.data_ptr(), ws.numel()))
+    return clip, table
 
 
 def global_norm(xs, max_norm=float("inf")):
     """[norm over all elements of the tensors, the coefficient that clips it to max_norm], on the device."""
-    px, ns, n = _arrays(xs, "global_norm")
-    clip = _clip(xs)
-    L = capi.lib()
-    ws = _ws(L.ag_global_norm_f32_workspace(n, ns), clip)
-    check(L.ag_global_norm_f32(_stream(), n, px, ns, max_norm, _ptr(clip), _ptr(ws), ws.numel()))
-    return clip
+    return _global_norm(xs, _sizes(xs, "global_norm"), max_norm)[0]
 
 
 def clip_by_global_norm(xs, max_norm, outs=None):
     """(outs, clip): the tensors times clip[1]; `outs` may be the tensors themselves (default: new ones)."""
-    px, ns, n = _arrays(xs, "clip_by_global_norm")
+    ns = _sizes(xs, "clip_by_global_norm")
     if outs is None:
         outs = [torch.empty_like(x) for x in xs]
-    po, no, m = _arrays(outs, "clip_by_global_norm")
-    if n != m or ns[:n] != no[:m]:
+    elif _sizes(outs, "clip_by_global_norm") != ns:
         raise capi.IncompatibleShape("clip_by_global_norm: outputs and inputs differ in number or size")
-    clip = _clip(xs)
-    L = capi.lib()
-    ws = _ws(L.ag_global_norm_f32_workspace(n, ns), clip)
-    check(L.ag_clip_by_global_norm_f32(_stream(), n, px, po, ns, max_norm, _ptr(clip), _ptr(ws), ws.numel()))
+    table, clip, ws = _norm_call(xs, ns)
+    check(capi.lib().ag_clip_by_global_norm_f32(_stream(), len(ns), _pointers(xs), _pointers(outs), table, max_norm, clip.data_ptr(), ws.data_ptr(),
+                                                ws.numel()))
     return outs, clip
 
 
 def adam_update_clipped(params, grads, ms, vs, ts, max_norm, alpha=1e-3, eps=1e-8, b1=0.9, b2=0.999):
     """One optimizer step on gradients clipped to max_norm over all of them, in place on params, ms, vs, ts (any number of
     parameters); the gradients themselves are left as they are.  Returns [norm, coefficient] on the device."""
-    n = len(params)
-    assert len(grads) == len(ms) == len(vs) == len(ts) == n
-    clip = global_norm(grads, max_norm)
-    tables = [_arrays(xs, "adam") for xs in (params, grads, ms, vs, ts)]
-    ns = tables[0][1]
-    if any(t[1][:n] != ns[:n] for t in tables[:4]) or any(t < 1 for t in tables[4][1][:n]):
+    ns = _sizes(grads, "adam")
+    if any(_sizes(xs, "adam") != ns for xs in (params, ms, vs)) or len(ts) != len(ns) or any(t < 1 for t in _sizes(ts, "adam")):
         raise capi.IncompatibleShape("adam: parameter, gradient and moment sizes differ")
+    clip, table = _global_norm(grads, ns, max_norm)
+    tables = [_pointers(xs) for xs in (params, grads, ms, vs, ts)] + [table]
     L = capi.lib()
-    most, word, st, pc = L.ag_adam_update_multi_max(), C.sizeof(C.c_void_p), _stream(), _ptr(clip)
+    n, most, word, st, pc = len(ns), L.ag_adam_update_multi_max(), C.sizeof(C.c_void_p), _stream(), clip.data_ptr()
     for i in range(0, n, most):
-        at = [C.byref(t[0], i * word) for t in tables]
-        check(L.ag_adam_update_multi_clipped_f32(st, min(most, n - i), *at, C.byref(ns, i * word), alpha, eps, b1, b2, pc))
+        check(L.ag_adam_update_multi_clipped_f32(st, min(most, n - i), *[C.byref(t, i * word) for t in tables], alpha, eps, b1, b2, pc))
     return clip

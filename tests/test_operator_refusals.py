@@ -127,3 +127,16 @@ def test_clipped_adam(L):
     refused(L, f(N, 1, t, table(8192), table(12288), table(16384), table(20480), one, 1e-3, 1e-8, 0.9, 0.999, N), 4, "clipping coefficient")
     refused(L, f(N, 99, t, t, t, t, t, one, 1e-3, 1e-8, 0.9, 0.999, P), 4, "at most")
     refused(L, f(N, 1, t, table(8192), table(12288), table(16384), table(None), one, 1e-3, 1e-8, 0.9, 0.999, P), 4, "step counter")
+
+
+def test_launchers_refuse_what_is_not_an_f32_tensor_of_the_device(capi):
+    """kernels.py looks at its arguments before anything is launched; a CPU tensor is the one that can be made anywhere."""
+    import torch
+    from rust_autograd_amd import kernels as K
+
+    x, e = torch.zeros(2, 8), None
+    for call in (lambda: K.quantize_e4m3(x), lambda: K.quantize_e4m3_both(x), lambda: K.rms_norm(x, x[0]), lambda: K.rms_norm_e4m3(x, x[0]),
+                 lambda: K.rms_norm_grad(x, x[0], x[0], x), lambda: K.quantize_matmul_e4m3(x, e), lambda: K.matmul_e4m3(e, e),
+                 lambda: K.matmul_e4m3(K.E4m3(x, x, 8), K.E4m3(x, x, 8))):
+        with pytest.raises(capi.TypeUnsupported):
+            call()
