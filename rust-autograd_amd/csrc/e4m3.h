@@ -16,12 +16,14 @@ inline size_t e4m3_scale_pitch(int n) { return (e4m3_pitch(n) / kE4m3Block + 3) 
 typedef float quad_t __attribute__((ext_vector_type(4)));
 typedef float quad_any_t __attribute__((ext_vector_type(4), aligned(4)));
 
-// Elements i..i+3 of a row of n, zeros behind its end.
+// Elements i..i+3 of a row of n, zeros behind its end.  STREAM: of an array that no cache will hold until it is read again.
+template <bool STREAM = false>
 __device__ inline quad_t load_quad(const float *row, long long i, long long n)
 {
     quad_t v = {0.f, 0.f, 0.f, 0.f};
     if (i + 4 <= n) {
-        v = *reinterpret_cast<const quad_any_t *>(row + i);
+        const quad_any_t *at = reinterpret_cast<const quad_any_t *>(row + i);
+        v = STREAM ? __builtin_nontemporal_load(at) : *at;
     } else {
 #pragma unroll
         for (int j = 0; j < 3; ++j)
@@ -29,10 +31,13 @@ __device__ inline quad_t load_quad(const float *row, long long i, long long n)
     }
     return v;
 }
+template <bool STREAM = false>
 __device__ inline void store_quad(float *row, long long i, long long n, quad_t v)
 {
     if (i + 4 <= n) {
-        *reinterpret_cast<quad_any_t *>(row + i) = v;
+        quad_any_t *at = reinterpret_cast<quad_any_t *>(row + i);
+        if (STREAM) __builtin_nontemporal_store(v, at);
+        else *at = v;
     } else {
 #pragma unroll
         for (int j = 0; j < 3; ++j)

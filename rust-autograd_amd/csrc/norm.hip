@@ -53,7 +53,7 @@ __device__ inline double square_sum(quad_t h, double s)
 // of the half wave hold between them (all of them call this together: the maximum runs over the half wave).
 __device__ inline void norm_write(const NormArgs &a, size_t row, long long i, quad_t y)
 {
-    if (a.y && i < a.n) store_quad(a.y + row * a.n, i, a.n, y);
+    if (a.y && i < a.n) store_quad<true>(a.y + row * a.n, i, a.n, y);
     if (a.q) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -67,7 +67,11 @@ __device__ inline void norm_write(const NormArgs &a, size_t row, long long i, qu
 
 // One row per T threads, held in registers (Q quads a thread: rows of up to 4 * Q * T elements), so every input is read
 // once; T = 64 packs four rows into a block of 256.  Behind the row's end quads are zero: they pad the 8-bit output.
-template <int T, int Q>
+// Bound by HBM: 16384 x 8192 with residual and 8-bit output 304 us (5.7 TB/s; a copy of 4 GiB reaches 4.7), of which
+// streaming stores give 11 and streaming loads 5 us; one row of 4096 5.2 us.  Stores stream always (1024 x 4096: 9.7 and
+// 12.5 us), loads from kStreamBytes on, beyond what the last-level cache keeps between two kernels (4096 x 4096, whose
+// arrays it does keep: 36 us without, 39 with; 16384 x 4096: 151 and 139).
+template <int T, int Q, bool STREAM>
 __global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_kernel(NormArgs a, unsigned rows)
 {
     __shared__ double part[T / 64];
@@ -78,11 +82,11 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_kernel(NormArgs a,
     const float *res = a.residual ? a.residual + row * a.n : nullptr;
     quad_t h[Q], w[Q];
 #pragma unroll
-    for (int k = 0; k < Q; ++k) h[k] = load_quad(x, (long long)(k * T + t) * 4, a.n);
+    for (int k = 0; k < Q; ++k) h[k] = load_quad<STREAM>(x, (long long)(k * T + t) * 4, a.n);
     if (res) {
         quad_t b[Q];
 #pragma unroll
-        for (int k = 0; k < Q; ++k) b[k] = load_quad(res, (long long)(k * T + t) * 4, a.n);
+        for (int k = 0; k < Q; ++k) b[k] = load_quad<STREAM>(res, (long long)(k * T + t) * 4, a.n);
 #pragma unroll
         for (int k = 0; k < Q; ++k) h[k] += b[k];
     }
@@ -97,7 +101,7 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_kernel(NormArgs a,
 #pragma unroll
     for (int k = 0; k < Q; ++k) {
         const long long i = (long long)(k * T + t) * 4;
-        if (a.h && i < a.n) store_quad(a.h + row * a.n, i, a.n, h[k]);
+        if (a.h && i < a.n) store_quad<true>(a.h + row * a.n, i, a.n, h[k]);
         norm_write(a, row, i, norm_quad(h[k], w[k], r));
     }
 }
@@ -130,6 +134,8 @@ __global__ __launch_bounds__(kLongT) void rms_norm_long_kernel(NormArgs a)
 }
 
 // ---- gradient ---------------------------------------------------------------------------------------------------------
+constexpr size_t kStreamBytes = (size_t)256 << 20;  // of one array
+
 struct NormGradArgs {
     const float *h, *weight, *rstd, *gy, *gh;
     float *gx, *partial;  // partial: [gridDim.x][n] sums of gw, or null
@@ -150,13 +156,17 @@ __device__ inline quad_t grad_quad(quad_t h, quad_t w, quad_t g, float r, float 
     return o;
 }
 
-// A block walks the rows b, b + G, ... with the row in registers and its share of gw beside it: gw costs one [G][n]
-// array of partial sums, folded in a fixed order below, instead of a second pass over gy and h.
-template <int T, int Q>
-__global__ __launch_bounds__(T) void rms_norm_grad_kernel(NormGradArgs a, unsigned rows)
+// A group of T threads walks rows in steps of the number of groups, with the row in registers and its share of gw beside
+// it: gw costs one [G][n] array of partial sums, folded in a fixed order below, instead of a second pass over gy and h.
+// T = 64: four groups share a block of 256 and add their sums through LDS at the end.  Bound by HBM: 16384 x 4096 with gh
+// 192 us, the fold included (5.6 TB/s; without streaming stores and loads 200).
+template <int T, int Q, bool STREAM>
+__global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_grad_kernel(NormGradArgs a, unsigned rows)
 {
+    constexpr unsigned PER = T == 64 ? 4 : 1;
     __shared__ double part[2][T / 64];
-    const unsigned t = threadIdx.x;
+    __shared__ quad_t sums[T == 64 ? 4 : 1][T == 64 ? Q * 64 : 1];
+    const unsigned t = T == 64 ? threadIdx.x & 63u : threadIdx.x, group = T == 64 ? threadIdx.x >> 6 : 0;
     quad_t w[Q], acc[Q];
 #pragma unroll
     for (int k = 0; k < Q; ++k) {
@@ -164,13 +174,13 @@ __global__ __launch_bounds__(T) void rms_norm_grad_kernel(NormGradArgs a, unsign
         acc[k] = quad_t{0.f, 0.f, 0.f, 0.f};
     }
     int turn = 0;
-    for (size_t row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
+    for (size_t row = (size_t)blockIdx.x * PER + group; row < rows; row += (size_t)gridDim.x * PER, turn ^= 1) {
         const float *hr = a.h + row * a.n, *gr = a.gy + row * a.n;
         quad_t h[Q], g[Q];
 #pragma unroll
         for (int k = 0; k < Q; ++k) {
-            h[k] = load_quad(hr, (long long)(k * T + t) * 4, a.n);
-            g[k] = load_quad(gr, (long long)(k * T + t) * 4, a.n);
+            h[k] = load_quad<STREAM>(hr, (long long)(k * T + t) * 4, a.n);
+            g[k] = load_quad<STREAM>(gr, (long long)(k * T + t) * 4, a.n);
         }
         const float r = a.rstd[row];
         double s = 0.0;
@@ -183,15 +193,22 @@ __global__ __launch_bounds__(T) void rms_norm_grad_kernel(NormGradArgs a, unsign
             const long long i = (long long)(k * T + t) * 4;
             if (a.gx && i < a.n) {
                 quad_t o = grad_quad(h[k], w[k], g[k], r, c);
-                if (a.gh) o += load_quad(a.gh + row * a.n, i, a.n);
-                store_quad(a.gx + row * a.n, i, a.n, o);
+                if (a.gh) o += load_quad<STREAM>(a.gh + row * a.n, i, a.n);
+                store_quad<true>(a.gx + row * a.n, i, a.n, o);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[k][j] = fmaf(g[k][j], h[k][j] * r, acc[k][j]);
         }
     }
-    if (a.partial) {
-        float *p = a.partial + (size_t)blockIdx.x * a.n;
+    if (!a.partial) return;
+    float *p = a.partial + (size_t)blockIdx.x * a.n;
+    if (T == 64) {
+#pragma unroll
+        for (int k = 0; k < Q; ++k) sums[group][k * 64 + t] = acc[k];
+        __syncthreads();
+        for (unsigned i = threadIdx.x; i < Q * 64; i += 256)
+            if ((long long)i * 4 < a.n) store_quad(p, (long long)i * 4, a.n, ((sums[0][i] + sums[1][i]) + sums[2][i]) + sums[3][i]);
+    } else {
 #pragma unroll
         for (int k = 0; k < Q; ++k) {
             const long long i = (long long)(k * T + t) * 4;
@@ -232,41 +249,49 @@ __global__ __launch_bounds__(kLongT) void rms_norm_grad_long_kernel(NormGradArgs
     }
 }
 
-// gw[c] = sum over the G partial rows, in 64 bits: 8 groups of 32 threads take every eighth row each (a quad of columns
+// gw[c] = sum over the G partial rows, in 64 bits: 32 groups of 32 threads take every 32nd row each (a quad of columns
 // per thread), and the groups are added in order.
-__global__ __launch_bounds__(256) void rms_norm_grad_fold_kernel(const float *__restrict__ partial, float *__restrict__ gw, long long n, unsigned G)
+constexpr int kFoldGroups = 32;
+__global__ __launch_bounds__(kFoldGroups * 32) void rms_norm_grad_fold_kernel(const float *__restrict__ partial, float *__restrict__ gw, long long n,
+                                                                             unsigned G)
 {
-    __shared__ double sums[8][32][4];
+    __shared__ double sums[kFoldGroups][128];
     const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
     const long long i = ((long long)blockIdx.x * 32 + lane) * 4;
     double s[4] = {0.0, 0.0, 0.0, 0.0};
     if (i < n)
 #pragma unroll 4
-        for (unsigned b = g; b < G; b += 8) {
+        for (unsigned b = g; b < G; b += kFoldGroups) {
             const quad_t v = load_quad(partial + (size_t)b * n, i, n);
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[j] += (double)v[j];
         }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sums[g][lane][j] = s[j];
+    for (int j = 0; j < 4; ++j) sums[g][lane * 4 + j] = s[j];
     __syncthreads();
-    if (g == 0 && i < n) {
-        quad_t o;
+    const long long c = (long long)blockIdx.x * 128 + threadIdx.x;
+    if (threadIdx.x < 128 && c < n) {
+        double t = sums[0][threadIdx.x];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            double t = sums[0][lane][j];
-#pragma unroll
-            for (int k = 1; k < 8; ++k) t += sums[k][lane][j];
-            o[j] = (float)t;
-        }
-        store_quad(gw, i, n, o);
+        for (int k = 1; k < kFoldGroups; ++k) t += sums[k][threadIdx.x];
+        gw[c] = (float)t;
     }
 }
 
 constexpr int kMaxRegisterRow = 4 * 8 * 1024;
 
 // Blocks that share the rows of a gradient: two per CU, at most one per row.
-inline unsigned norm_grad_blocks(long long rows) { return (unsigned)(rows < 2LL * device_cus() ? rows : 2LL * device_cus()); }
+// Rows of up to this many elements have a wave each in the gradient: 65536 x 512 takes 111 us, 200000 x 128 102, with a
+// block of 256 each 227 and 718.
+constexpr int kWaveRow = 1024;
+
+// Blocks that share the rows of a gradient: two per CU (three: 8192 x 4096 208 us for both directions, two: 203), of one
+// row at a time or, where a wave has a row, four; not more than there are rows.
+inline unsigned norm_grad_blocks(long long rows, int n)
+{
+    const long long groups = n <= kWaveRow ? (rows + 3) / 4 : rows, most = (n <= kWaveRow ? 8LL : 2LL) * device_cus();
+    return (unsigned)(groups < most ? groups : most);
+}
 
 }  // namespace ag
 
@@ -288,7 +313,12 @@ extern "C" ag_status_t ag_rms_norm_f32(ag_stream_t stream, const float *x, const
     const unsigned R = (unsigned)rows;
     // Threads of a row: the padding of the scales (a multiple of 512 elements) has to be covered by the quads.
     const long long cells = (long long)e4m3_scale_pitch(n) * kE4m3Block;
-#define NORM(T, Q) hipLaunchKernelGGL((rms_norm_kernel<T, Q>), dim3(T == 64 ? (R + 3) / 4 : R), dim3(T == 64 ? 256 : T), 0, st, a, R)
+    const bool streams = (size_t)rows * (size_t)n * sizeof(float) >= kStreamBytes;
+#define NORM(T, Q)                                                                                                             \
+    do {                                                                                                                       \
+        if (streams) hipLaunchKernelGGL((rms_norm_kernel<T, Q, true>), dim3(T == 64 ? (R + 3) / 4 : R), dim3(T == 64 ? 256 : T), 0, st, a, R); \
+        else hipLaunchKernelGGL((rms_norm_kernel<T, Q, false>), dim3(T == 64 ? (R + 3) / 4 : R), dim3(T == 64 ? 256 : T), 0, st, a, R);       \
+    } while (0)
     if (cells <= 512) NORM(64, 2);
     else if (cells <= 1024) NORM(64, 4);
     else if (cells <= 2048) NORM(256, 2);
@@ -304,7 +334,7 @@ extern "C" ag_status_t ag_rms_norm_f32(ag_stream_t stream, const float *x, const
 extern "C" size_t ag_rms_norm_grad_f32_workspace(int rows, int n)
 {
     if (rows <= 0 || n <= 0) return 0;
-    return (size_t)norm_grad_blocks(rows) * (size_t)n * sizeof(float);
+    return (size_t)norm_grad_blocks(rows, n) * (size_t)n * sizeof(float);
 }
 
 extern "C" ag_status_t ag_rms_norm_grad_f32(ag_stream_t stream, const float *h, const float *weight, const float *rstd, const float *gy,
@@ -323,10 +353,17 @@ extern "C" ag_status_t ag_rms_norm_grad_f32(ag_stream_t stream, const float *h, 
     AG_REQUIRE(!gw || (ws && ws_bytes >= ag_rms_norm_grad_f32_workspace(rows, n)), AG_ERR_INVALID_DIMS,
                "rms_norm_grad: workspace of %zu bytes, %zu needed", ws_bytes, ag_rms_norm_grad_f32_workspace(rows, n));
     AG_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 3u) == 0, AG_ERR_INVALID_DIMS, "rms_norm_grad: misaligned workspace");
-    const unsigned R = (unsigned)rows, G = norm_grad_blocks(rows);
+    const unsigned R = (unsigned)rows, G = norm_grad_blocks(rows, n);
     NormGradArgs a = {h, weight, rstd, gy, gh, gx, gw ? static_cast<float *>(ws) : nullptr, n};
-#define GRAD(T, Q) hipLaunchKernelGGL((rms_norm_grad_kernel<T, Q>), dim3(G), dim3(T), 0, st, a, R)
-    if (n <= 1024) GRAD(256, 1);
+    const bool streams = (size_t)rows * (size_t)n * sizeof(float) >= kStreamBytes;
+#define GRAD(T, Q)                                                                                                            \
+    do {                                                                                                                      \
+        if (streams) hipLaunchKernelGGL((rms_norm_grad_kernel<T, Q, true>), dim3(G), dim3(T == 64 ? 256 : T), 0, st, a, R);    \
+        else hipLaunchKernelGGL((rms_norm_grad_kernel<T, Q, false>), dim3(G), dim3(T == 64 ? 256 : T), 0, st, a, R);          \
+    } while (0)
+    if (n <= 256) GRAD(64, 1);
+    else if (n <= 512) GRAD(64, 2);
+    else if (n <= kWaveRow) GRAD(64, 4);
     else if (n <= 2048) GRAD(256, 2);
     else if (n <= 4096) GRAD(256, 4);
     else if (n <= 8192) GRAD(512, 4);
@@ -337,6 +374,7 @@ extern "C" ag_status_t ag_rms_norm_grad_f32(ag_stream_t stream, const float *h, 
     }
 #undef GRAD
     if (gw)
-        hipLaunchKernelGGL(rms_norm_grad_fold_kernel, dim3((unsigned)((n + 127) / 128)), dim3(256), 0, st, static_cast<const float *>(ws), gw, n, G);
+        hipLaunchKernelGGL(rms_norm_grad_fold_kernel, dim3((unsigned)((n + 127) / 128)), dim3(kFoldGroups * 32), 0, st,
+                           static_cast<const float *>(ws), gw, n, G);
     return check_launch("rms_norm_grad");
 }
