@@ -45,12 +45,12 @@ __device__ inline void store_quad(float *row, long long i, long long n, quad_t v
     }
 }
 
-// The bits of |v| where v is finite, 0 where it is not: their integer maximum is that of the finite magnitudes.
-__device__ inline unsigned finite_magnitude(float v)
-{
-    const unsigned b = __float_as_uint(v) & 0x7fffffffu;
-    return b < 0x7f800000u ? b : 0u;
-}
+// The bits of |v|: their integer order is that of the magnitudes, and from kNotFinite on they are an infinity or a NaN.
+constexpr unsigned kNotFinite = 0x7f800000u;
+__device__ inline unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ inline unsigned magnitude(quad_t v) { return max(max(magnitude(v[0]), magnitude(v[1])), max(magnitude(v[2]), magnitude(v[3]))); }
+// The same with 0 for what is not finite.
+__device__ inline unsigned finite_magnitude(float v) { return magnitude(v) < kNotFinite ? magnitude(v) : 0u; }
 __device__ inline unsigned finite_magnitude(quad_t v)
 {
     return max(max(finite_magnitude(v[0]), finite_magnitude(v[1])), max(finite_magnitude(v[2]), finite_magnitude(v[3])));
@@ -66,27 +66,45 @@ __device__ inline unsigned scale_byte(unsigned amax)
 }
 __device__ inline float scale_inverse(unsigned byte) { return __uint_as_float((254u - byte) << 23); }
 
-// Four values times `inv`, rounded to e4m3 (to nearest, ties to even; |v| * inv <= 448).  e4m3 has no infinities: values
-// that are not finite become NaN.
-__device__ inline unsigned round_e4m3(quad_t v, float inv)
+// Four finite values times `inv`, rounded to e4m3 (to nearest, ties to even; |v| * inv <= 448).
+__device__ inline unsigned round_finite(quad_t v, float inv)
 {
-    float s[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const bool finite = (__float_as_uint(v[j]) & 0x7fffffffu) < 0x7f800000u;
-        s[j] = finite ? v[j] * inv : __uint_as_float(0x7fc00000u);
-    }
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(s[0], s[1], 0, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(s[2], s[3], w, true);
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, w, true);
     return (unsigned)w;
 }
-
-// Maximum over the 32 lanes of a half wave (every lane gets it).
-__device__ inline unsigned half_wave_max(unsigned v)
+// Any four values: e4m3 has no infinities, what is not finite becomes NaN.
+__device__ inline unsigned round_any(quad_t v, float inv)
 {
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, d, 64));
-    return v;
+    for (int j = 0; j < 4; ++j)
+        if (magnitude(v[j]) >= kNotFinite) v[j] = __uint_as_float(0x7fc00000u);
+    return round_finite(v, inv);
+}
+
+// Maximum over the 32 lanes of a half wave (every lane gets it): four rotations within the rows of 16 lanes, which cost an
+// instruction each, and one exchange between the two rows.
+__device__ inline unsigned half_wave_max(unsigned v)
+{
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x124, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x122, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x121, 0xf, 0xf, false));
+    return max(v, (unsigned)__builtin_amdgcn_ds_swizzle((int)v, 0x401f));
+}
+
+// A block of 128 that the 32 lanes of a half wave hold, a quad each: its scale byte, and the lane's four values.  (All 32
+// lanes come here together.  Blocks with infinities or NaN, which take no part in the scale, are gone over twice.)
+__device__ inline unsigned round_block(quad_t v, unsigned *byte)
+{
+    unsigned top = half_wave_max(magnitude(v));
+    if (__builtin_expect(top < kNotFinite, 1)) {
+        *byte = scale_byte(top);
+        return round_finite(v, scale_inverse(*byte));
+    }
+    top = half_wave_max(finite_magnitude(v));
+    *byte = scale_byte(top);
+    return round_any(v, scale_inverse(*byte));
 }
 #endif
 

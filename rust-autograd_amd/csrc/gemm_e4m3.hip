@@ -349,8 +349,8 @@ __global__ __launch_bounds__(NW * 64) void gemm_e4m3_skinny_kernel(GemmE4m3 p, c
                 for (int r = 0; r < ROWS; ++r)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const unsigned sb = scale_byte(half_wave_max(finite_magnitude(v[r][i])));
-                        *reinterpret_cast<unsigned *>(&rounded[wave][r][(half + 2 * i) * 128 + l31 * 4]) = round_e4m3(v[r][i], scale_inverse(sb));
+                        unsigned sb;
+                        *reinterpret_cast<unsigned *>(&rounded[wave][r][(half + 2 * i) * 128 + l31 * 4]) = round_block(v[r][i], &sb);
                         if (l31 == 0) rounded_scales[wave][r][half + 2 * i] = (unsigned char)sb;
                     }
             };

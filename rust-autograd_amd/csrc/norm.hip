@@ -58,9 +58,10 @@ __device__ inline void norm_write(const NormArgs &a, size_t row, long long i, qu
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (i + j >= a.n) y[j] = 0.f;  // (padding stays zero where r is not finite)
-        const unsigned sb = scale_byte(half_wave_max(finite_magnitude(y)));
+        unsigned sb;
+        const unsigned bytes = round_block(y, &sb);
         const long long b = i / kE4m3Block;
-        if (b < a.nb) *reinterpret_cast<unsigned *>(a.q + (row * a.nb) * kE4m3Block + i) = round_e4m3(y, scale_inverse(sb));
+        if (b < a.nb) *reinterpret_cast<unsigned *>(a.q + (row * a.nb) * kE4m3Block + i) = bytes;
         if ((threadIdx.x & 31) == 0 && b < a.nbp) a.scales[row * a.nbp + b] = (unsigned char)sb;
     }
 }

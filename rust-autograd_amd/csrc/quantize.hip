@@ -6,7 +6,8 @@ namespace ag {
 
 // Along the rows.  32 lanes hold one block of 128 elements, a quad each: its largest magnitude is a maximum over the
 // half wave, and the block leaves as 32 x 4 bytes = one 128-byte line.  Blocks are independent, so the kernel is one
-// stream: 4 bytes in, 1 byte and 1/128 out per element.  Block columns nb..scale_pitch are padding: scale 1, no data.
+// stream, bound by HBM: 4 bytes in, 1 byte and 1/128 out per element; 16384 x 8192 117 us (5.8 TB/s).  Block columns
+// nb..scale_pitch are padding: scale 1, no data.
 constexpr int kRowsPerThread = 4;
 
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const float *__restrict__ x, long long ldx, int cols, unsigned char *__restrict__ q,
@@ -26,10 +27,10 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const float *__restr
     }
 #pragma unroll
     for (int i = 0; i < kRowsPerThread; ++i) {
-        const unsigned sb = scale_byte(half_wave_max(finite_magnitude(v[i])));
+        unsigned sb;
+        const unsigned bytes = round_block(v[i], &sb);
         if (first + i >= items) continue;
-        if (b[i] < nb)
-            *reinterpret_cast<unsigned *>(q + ((size_t)row[i] * nb + b[i]) * kE4m3Block + lane * 4) = round_e4m3(v[i], scale_inverse(sb));
+        if (b[i] < nb) *reinterpret_cast<unsigned *>(q + ((size_t)row[i] * nb + b[i]) * kE4m3Block + lane * 4) = bytes;
         if (lane == 0) scales[(size_t)row[i] * nbp + b[i]] = (unsigned char)sb;
     }
 }
@@ -39,13 +40,16 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const float *__restr
 // a column's one over the thread's rows and then over the 8 groups through LDS.  The 16 values that a thread rounds for a
 // column are 16 consecutive bytes of the transposed array; they pass through LDS so that each column leaves as one
 // 128-byte line.  (LDS pitch 144 = 128 + 16: the 16-byte pieces of a thread's four columns fall on different banks.)
+// 16384 x 8192: 164 us both ways (4.9 TB/s of 6 bytes an element; one way after the other 117 + 140), 8192 x 4096 42 us.
+// With the half wave's maxima exchanged through LDS and each value tested for being finite the arithmetic bound it: 199
+// and 54 us.
 __global__ __launch_bounds__(256) void quantize_tile_kernel(const float *__restrict__ x, long long ldx, int rows, int cols,
                                                             unsigned char *__restrict__ q, unsigned char *__restrict__ scales,
                                                             unsigned char *__restrict__ qt, unsigned char *__restrict__ scales_t, unsigned nb,
                                                             unsigned nbp, unsigned mb, unsigned mbp)
 {
     constexpr int kPitch = kE4m3Block + 16;
-    __shared__ unsigned colmax[8][kE4m3Block];
+    __shared__ __attribute__((aligned(16))) unsigned colmax[8][kE4m3Block];
     __shared__ __attribute__((aligned(16))) unsigned char turned[kE4m3Block * kPitch];
     const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
     const unsigned tb = blockIdx.x % nb, tm = blockIdx.x / nb;  // block column, block row
@@ -57,21 +61,34 @@ __global__ __launch_bounds__(256) void quantize_tile_kernel(const float *__restr
         v[i] = quad_t{0.f, 0.f, 0.f, 0.f};
         if (m0 + i < rows) v[i] = load_quad(x + (m0 + i) * ldx, c0 + lane * 4, cols);
     }
-    unsigned cm[4] = {0, 0, 0, 0};
+    unsigned top[4];  // of this thread's columns
+    auto column_maxima = [&](auto magnitude_of) {
+        unsigned cm[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+        for (int i = 0; i < 16; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) cm[j] = max(cm[j], finite_magnitude(v[i][j]));
+            for (int j = 0; j < 4; ++j) cm[j] = max(cm[j], magnitude_of(v[i][j]));
+        *reinterpret_cast<uint4 *>(&colmax[g][lane * 4]) = make_uint4(cm[0], cm[1], cm[2], cm[3]);
+        __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) colmax[g][lane * 4 + j] = cm[j];
-    __syncthreads();
+        for (int j = 0; j < 4; ++j) top[j] = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint4 c = *reinterpret_cast<const uint4 *>(&colmax[k][lane * 4]);
+            top[0] = max(top[0], c.x);
+            top[1] = max(top[1], c.y);
+            top[2] = max(top[2], c.z);
+            top[3] = max(top[3], c.w);
+        }
+    };
+    column_maxima([](float x) { return magnitude(x); });
+    // (every thread sees the maxima of its own columns only: the block agrees)
+    const bool finite = !__syncthreads_or(max(max(top[0], top[1]), max(top[2], top[3])) >= kNotFinite);
+    if (!finite) column_maxima([](float x) { return finite_magnitude(x); });
     float inv[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        unsigned top = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) top = max(top, colmax[k][lane * 4 + j]);
-        const unsigned sb = scale_byte(top);
+        const unsigned sb = scale_byte(top[j]);
         inv[j] = scale_inverse(sb);
         const long long c = c0 + lane * 4 + j;
         if (g == 0 && c < cols) {
@@ -80,21 +97,26 @@ __global__ __launch_bounds__(256) void quantize_tile_kernel(const float *__restr
                 for (unsigned k = mb; k < mbp; ++k) scales_t[c * mbp + k] = 127;
         }
     }
+    auto turn = [&](auto round) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        uint4 w;
-        w.x = round_e4m3(quad_t{v[0][j], v[1][j], v[2][j], v[3][j]}, inv[j]);
-        w.y = round_e4m3(quad_t{v[4][j], v[5][j], v[6][j], v[7][j]}, inv[j]);
-        w.z = round_e4m3(quad_t{v[8][j], v[9][j], v[10][j], v[11][j]}, inv[j]);
-        w.w = round_e4m3(quad_t{v[12][j], v[13][j], v[14][j], v[15][j]}, inv[j]);
-        *reinterpret_cast<uint4 *>(turned + (lane * 4 + j) * kPitch + g * 16) = w;
-    }
+        for (int j = 0; j < 4; ++j) {
+            uint4 w;
+            w.x = round(quad_t{v[0][j], v[1][j], v[2][j], v[3][j]}, inv[j]);
+            w.y = round(quad_t{v[4][j], v[5][j], v[6][j], v[7][j]}, inv[j]);
+            w.z = round(quad_t{v[8][j], v[9][j], v[10][j], v[11][j]}, inv[j]);
+            w.w = round(quad_t{v[12][j], v[13][j], v[14][j], v[15][j]}, inv[j]);
+            *reinterpret_cast<uint4 *>(turned + (lane * 4 + j) * kPitch + g * 16) = w;
+        }
+    };
+    if (finite) turn([](quad_t x, float s) { return round_finite(x, s); });
+    else turn([](quad_t x, float s) { return round_any(x, s); });
     if (q) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const unsigned sb = scale_byte(half_wave_max(finite_magnitude(v[i])));
+            unsigned sb;
+            const unsigned bytes = round_block(v[i], &sb);
             if (m0 + i >= rows) continue;
-            *reinterpret_cast<unsigned *>(q + ((size_t)(m0 + i) * nb + tb) * kE4m3Block + lane * 4) = round_e4m3(v[i], scale_inverse(sb));
+            *reinterpret_cast<unsigned *>(q + ((size_t)(m0 + i) * nb + tb) * kE4m3Block + lane * 4) = bytes;
             if (lane == 0) {
                 scales[(size_t)(m0 + i) * nbp + tb] = (unsigned char)sb;
                 if (tb == nb - 1)
