@@ -221,7 +221,7 @@ static ag_status_t launch_norm(hipStream_t st, int count, const float *const *xs
 }
 
 // Blocks of one launch write what others of it read unless every output is its own input or apart from all of them.
-static ag_status_t clip_check_overlap(int count, const float *const *xs, float *const *outs, const size_t *ns)
+static ag_status_t clip_check_overlap(int count, const float *const *xs, float *const *outs, const size_t *ns, const float *clip)
 try {
     struct Range {
         uintptr_t from, to;
@@ -233,9 +233,12 @@ try {
     for (int i = 0; i < count; ++i) {
         if (ns[i] == 0) continue;
         AG_REQUIRE(outs[i], AG_ERR_INVALID_DIMS, "clip_by_global_norm: null pointer (array %d)", i);
-        const uintptr_t x = reinterpret_cast<uintptr_t>(xs[i]), o = reinterpret_cast<uintptr_t>(outs[i]);
-        ranges.push_back({o, o + ns[i] * sizeof(float), i, true});
-        if (x != o) ranges.push_back({x, x + ns[i] * sizeof(float), i, false});
+        const uintptr_t x = reinterpret_cast<uintptr_t>(xs[i]), o = reinterpret_cast<uintptr_t>(outs[i]), c = reinterpret_cast<uintptr_t>(clip);
+        const size_t bytes = ns[i] * sizeof(float);
+        AG_REQUIRE((c + 8 <= x || c >= x + bytes) && (c + 8 <= o || c >= o + bytes), AG_ERR_INVALID_DIMS,
+                   "clip_by_global_norm: array %d overlaps the norm and coefficient", i);
+        ranges.push_back({o, o + bytes, i, true});
+        if (x != o) ranges.push_back({x, x + bytes, i, false});
     }
     std::sort(ranges.begin(), ranges.end(), [](const Range &a, const Range &b) { return a.from < b.from; });
     // in the order of their starts: an output may overlap nothing, an input may overlap inputs
@@ -275,7 +278,7 @@ extern "C" ag_status_t ag_clip_by_global_norm_f32(ag_stream_t stream, int count,
     ag_status_t e = clip_check("clip_by_global_norm", count, xs, ns, max_norm, clip, ws, ws_bytes);
     if (e != AG_OK) return e;
     AG_REQUIRE(count == 0 || outs, AG_ERR_INVALID_DIMS, "clip_by_global_norm: null pointer table");
-    e = clip_check_overlap(count, xs, outs, ns);
+    e = clip_check_overlap(count, xs, outs, ns, clip);
     if (e != AG_OK) return e;
     hipStream_t st = as_stream(stream);
     e = launch_norm(st, count, xs, ns, max_norm, clip, static_cast<double *>(ws));

@@ -123,7 +123,10 @@ def test_rounding_reads_a_strided_view(K, rng):
 # extents around the tiles and blocks of the kernels, and the skinny ones
 PRODUCTS = [(1, 1, 1), (1, 17, 128), (1, 4096, 512), (2, 100, 300), (5, 33, 129), (16, 16, 128), (16, 1000, 4096), (17, 255, 640), (31, 64, 1000),
             (48, 129, 2048), (63, 500, 513), (64, 128, 128), (65, 127, 384), (128, 128, 1024), (129, 257, 130), (200, 1, 700), (255, 256, 257),
-            (256, 256, 256), (257, 513, 1100), (300, 2000, 8192), (512, 512, 640), (1000, 1999, 2500), (1024, 768, 128)]
+            (256, 256, 256), (257, 513, 1100), (300, 2000, 8192), (512, 512, 640), (1000, 1999, 2500), (1024, 768, 128), (30, 5000, 700),
+            (33, 4000, 4100), (20, 4096, 4096), (64, 300, 16400)]
+# tiles of 128 four steps and two steps deep and of 256, contractions of one to six steps
+PRODUCTS += [(m, n, k) for m, n in ((1030, 3900), (1990, 4000), (2100, 4400)) for k in (100, 256, 300, 512, 640, 768)]
 
 
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
@@ -241,3 +244,42 @@ def test_same_bits_on_another_stream_and_from_a_graph(K, rng, m, n, k):
         torch.cuda.synchronize()
         assert torch.equal(captured, want), f"replay {i}"
         assert torch.equal(second, two), f"replay {i}, in two calls"
+
+
+def test_offsets_beyond_32_bits(K, rng):
+    """2.4 * 10^9 elements: the last rows of the array come out as they do alone, in every form that reads or writes them."""
+    rows, k, last = 600_000, 4096, 70
+    tail = dev(rng.integers(-3, 4, (last, k)))
+    x = torch.zeros(rows, k, device="cuda")
+    x[-last:] = tail
+    small = dev(rng.integers(-3, 4, (40, k)))
+    qs, qtail = K.quantize_e4m3(small), K.quantize_e4m3(tail)
+    e = K.quantize_e4m3(x)
+    assert torch.equal(e.q[-last:].view(torch.uint8), qtail.q.view(torch.uint8)) and torch.equal(e.scales[-last:].view(torch.uint8), qtail.scales.view(torch.uint8))
+    want = (tail.double() @ small.double().t()).float()  # integers: exact in every order
+    assert torch.equal(K.matmul_e4m3(e, qs)[-last:], want)
+    assert torch.equal(K.matmul_e4m3(qs, e)[:, -last:], want.t())
+    one = K.quantize_matmul_e4m3(small[:1], e)
+    assert torch.equal(one[0, -last:], want[:, 0]) and not one[0, :-last].any()
+    del e, one
+    torch.cuda.empty_cache()
+    e, t = K.quantize_e4m3_both(x)
+    assert torch.equal(e.q[-last:].view(torch.uint8), qtail.q.view(torch.uint8))
+    assert not t.q[:, rows - last - 1000: rows - last].float().any()
+    # 600000 = 4687 * 128 + 64: the last block of a column holds the last 64 rows
+    got = host(t.q[:, 4687 * 128: rows]) * np.exp2(t.scales.view(torch.uint8)[:, 4687:4688].cpu().numpy().astype(np.float64) - 127)
+    assert np.array_equal(got, host(tail[-64:]).T)
+    del e, t
+    torch.cuda.empty_cache()
+    w = torch.ones(k, device="cuda")
+    y, h, rstd = K.rms_norm(x, w, 1e-6, residual=x)
+    y1, h1, rstd1 = K.rms_norm(tail, w, 1e-6, residual=tail)
+    assert torch.equal(y[-last:], y1) and torch.equal(h[-last:], h1) and torch.equal(rstd[-last:], rstd1)
+    gx, _ = K.rms_norm_grad(h, w, rstd, y)
+    gx1, _ = K.rms_norm_grad(h1, w, rstd1, y1)
+    assert torch.equal(gx[-last:], gx1)
+    del y, gx
+    outs, clip = K.clip_by_global_norm([x, h], 1.0, outs=[x, h])
+    norm = np.sqrt((host(tail) ** 2).sum() * 5)  # h is twice x
+    assert abs(host(clip)[0] - norm) <= 2.0 ** -24 * (1 + 1e-6) * norm
+    assert torch.equal(x[-last:], tail * clip[1]) and torch.equal(h[-last:], h1 * clip[1])

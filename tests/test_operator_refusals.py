@@ -56,6 +56,13 @@ def test_product(L):
     f = L.ag_matmul_e4m3_f32
     refused(L, f(N, 2, -2, 4, P, P, P, P, P, 4, P, 1 << 30), 4, "negative extent")
     refused(L, f(N, 2, 8, 4, P, P, P, P, P, 7, P, 1 << 30), 2, "ldc (7)")
+    refused(L, f(N, 2, 8, (1 << 28) + 1, P, P, P, P, P, 8, P, 1 << 30), 4, "at most 2^28")
+    refused(L, f(N, 2, 8, 4, P, C.c_void_p(4098), P, P, P, 8, P, 1 << 30), 4, "4-byte aligned")
+    refused(L, f(N, 2, 8, 4, P, P, P, C.c_void_p(4098), P, 8, P, 1 << 30), 4, "4-byte aligned")
+    need = L.ag_matmul_e4m3_f32_workspace(64, 1000, 8192)  # a contraction that is cut
+    assert need > 0
+    refused(L, f(N, 64, 1000, 8192, P, P, P, P, P, 1000, P, need - 1), 4, "workspace")
+    refused(L, f(N, 64, 1000, 8192, P, P, P, P, P, 1000, ODD, need), 4, "misaligned workspace")
     for a in ((N, P, P, P, P), (P, N, P, P, P), (P, P, N, P, P), (P, P, P, N, P), (P, P, P, P, N)):
         refused(L, f(N, 2, 8, 4, *a, 8, P, 1 << 30), 4, "null pointer")
     refused(L, f(N, 2, 8, 4, ODD, P, P, P, P, 8, P, 1 << 30), 4, "16-byte aligned")
@@ -112,13 +119,17 @@ def test_clipping(L):
     refused(L, f(N, 2, xs, ns, 1.0, P, P, need - 1), 4, "workspace")
     refused(L, f(N, 2, xs, ns, 1.0, P, C.c_void_p(4100), need), 4, "misaligned workspace")
     refused(L, c(N, 2, xs, N, ns, 1.0, P, P, need), 4, "null pointer table")
-    refused(L, c(N, 2, xs, table(4096, None), ns, 1.0, P, P, need), 4, "array 1")
+    refused(L, c(N, 2, xs, table(4096, None), ns, 1.0, C.c_void_p(1 << 20), P, need), 4, "array 1")
     # the same array twice in place, an output over another input, an output over another output, a shifted copy of itself
-    refused(L, c(N, 2, table(4096, 4096), table(4096, 4096), ns, 1.0, P, P, need), 4, "overlaps")
-    refused(L, c(N, 2, xs, table(16384, 4100), ns, 1.0, P, P, need), 4, "overlaps")
-    refused(L, c(N, 2, xs, table(16384, 16396), ns, 1.0, P, P, need), 4, "overlaps")
-    refused(L, c(N, 2, xs, table(4100, 16384), ns, 1.0, P, P, need), 4, "overlaps")
-    refused(L, c(N, 2, xs, table(4092, 16384), ns, 1.0, P, P, need), 4, "overlaps")
+    F = C.c_void_p(1 << 20)
+    refused(L, c(N, 2, table(4096, 4096), table(4096, 4096), ns, 1.0, F, P, need), 4, "overlaps")
+    refused(L, c(N, 2, xs, table(16384, 4100), ns, 1.0, F, P, need), 4, "overlaps")
+    refused(L, c(N, 2, xs, table(16384, 16396), ns, 1.0, F, P, need), 4, "overlaps")
+    refused(L, c(N, 2, xs, table(4100, 16384), ns, 1.0, F, P, need), 4, "overlaps")
+    refused(L, c(N, 2, xs, table(4092, 16384), ns, 1.0, F, P, need), 4, "overlaps")
+    # the norm and coefficient inside an input, inside an output
+    refused(L, c(N, 2, xs, table(16384, 32768), ns, 1.0, C.c_void_p(8200), P, need), 4, "array 1 overlaps the norm")
+    refused(L, c(N, 2, xs, table(16384, 32768), ns, 1.0, C.c_void_p(16380), P, need), 4, "array 0 overlaps the norm")
 
 
 def test_clipped_adam(L):
