@@ -53,7 +53,7 @@ __device__ inline double square_sum(quad_t h, double s)
 // of the half wave hold between them (all of them call this together: the maximum runs over the half wave).
 __device__ inline void norm_write(const NormArgs &a, size_t row, long long i, quad_t y)
 {
-    if (a.y && i < a.n) store_quad<true>(a.y + row * a.n, i, a.n, y);
+    if (a.y) store_quad<true>(a.y + row * a.n, i, a.n, y);
     if (a.q) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -68,10 +68,11 @@ __device__ inline void norm_write(const NormArgs &a, size_t row, long long i, qu
 
 // One row per T threads, held in registers (Q quads a thread: rows of up to 4 * Q * T elements), so every input is read
 // once; T = 64 packs four rows into a block of 256.  Behind the row's end quads are zero: they pad the 8-bit output.
-// Bound by HBM: 16384 x 8192 with residual and 8-bit output 304 us (5.7 TB/s; a copy of 4 GiB reaches 4.7), of which
-// streaming stores give 11 and streaming loads 5 us; one row of 4096 5.2 us.  Stores stream always (1024 x 4096: 9.7 and
+// Bound by HBM: 16384 x 8192 with residual and 8-bit output 270 us (6.4 TB/s; a copy of 4 GiB reaches 4.7; 16 us more
+// without streaming stores and loads, 15 with the half wave's maxima exchanged through LDS); one row of 4096 4.8 us.  Stores stream always (1024 x 4096: 9.7 and
 // 12.5 us), loads from kStreamBytes on, beyond what the last-level cache keeps between two kernels (4096 x 4096, whose
-// arrays it does keep: 36 us without, 39 with; 16384 x 4096: 151 and 139).
+// arrays it does keep: 36 us without, 39 with; 16384 x 4096: 151 and 139).  The quads of a thread come in small steps of
+// the row's length: 16384 x 5001 to 8 bits 202 us with 5 quads a thread, 233 with 8; its gradient 251 and 336.
 template <int T, int Q, bool STREAM>
 __global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_kernel(NormArgs a, unsigned rows)
 {
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_kernel(NormArgs a,
 #pragma unroll
     for (int k = 0; k < Q; ++k) {
         const long long i = (long long)(k * T + t) * 4;
-        if (a.h && i < a.n) store_quad<true>(a.h + row * a.n, i, a.n, h[k]);
+        if (a.h) store_quad<true>(a.h + row * a.n, i, a.n, h[k]);
         norm_write(a, row, i, norm_quad(h[k], w[k], r));
     }
 }
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_grad_kernel(NormGr
 #pragma unroll
         for (int k = 0; k < Q; ++k) {
             const long long i = (long long)(k * T + t) * 4;
-            if (a.gx && i < a.n) {
+            if (a.gx) {
                 quad_t o = grad_quad(h[k], w[k], g[k], r, c);
                 if (a.gh) o += load_quad<STREAM>(a.gh + row * a.n, i, a.n);
                 store_quad<true>(a.gx + row * a.n, i, a.n, o);
@@ -208,13 +209,10 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_grad_kernel(NormGr
         for (int k = 0; k < Q; ++k) sums[group][k * 64 + t] = acc[k];
         __syncthreads();
         for (unsigned i = threadIdx.x; i < Q * 64; i += 256)
-            if ((long long)i * 4 < a.n) store_quad(p, (long long)i * 4, a.n, ((sums[0][i] + sums[1][i]) + sums[2][i]) + sums[3][i]);
+            store_quad(p, (long long)i * 4, a.n, ((sums[0][i] + sums[1][i]) + sums[2][i]) + sums[3][i]);
     } else {
 #pragma unroll
-        for (int k = 0; k < Q; ++k) {
-            const long long i = (long long)(k * T + t) * 4;
-            if (i < a.n) store_quad(p, i, a.n, acc[k]);
-        }
+        for (int k = 0; k < Q; ++k) store_quad(p, (long long)(k * T + t) * 4, a.n, acc[k]);
     }
 }
 
@@ -250,15 +248,17 @@ __global__ __launch_bounds__(kLongT) void rms_norm_grad_long_kernel(NormGradArgs
     }
 }
 
-// gw[c] = sum over the G partial rows, in 64 bits: 32 groups of 32 threads take every 32nd row each (a quad of columns
-// per thread), and the groups are added in order.
-constexpr int kFoldGroups = 32;
-__global__ __launch_bounds__(kFoldGroups * 32) void rms_norm_grad_fold_kernel(const float *__restrict__ partial, float *__restrict__ gw, long long n,
-                                                                             unsigned G)
+// gw[c] = sum over the G partial rows, in 64 bits: a block has 32 columns, 128 groups of 8 threads take every 128th row
+// each (a quad of columns per thread), and the groups are added in order, by eights and then the sixteen sums.  (With 128
+// columns to a block and 32 groups a short row leaves most of the chip idle: the gradient
+// of 20000 x 257 takes 49 us that way and 27 this way, of 2000 x 1023 20 and 15.)
+constexpr int kFoldGroups = 128;
+__global__ __launch_bounds__(kFoldGroups * 8) void rms_norm_grad_fold_kernel(const float *__restrict__ partial, float *__restrict__ gw, long long n,
+                                                                            unsigned G)
 {
-    __shared__ double sums[kFoldGroups][128];
-    const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
-    const long long i = ((long long)blockIdx.x * 32 + lane) * 4;
+    __shared__ double sums[kFoldGroups][32], eights[kFoldGroups / 8][32];
+    const int lane = threadIdx.x & 7, g = threadIdx.x >> 3;
+    const long long i = ((long long)blockIdx.x * 8 + lane) * 4;
     double s[4] = {0.0, 0.0, 0.0, 0.0};
     if (i < n)
 #pragma unroll 4
@@ -270,12 +270,19 @@ __global__ __launch_bounds__(kFoldGroups * 32) void rms_norm_grad_fold_kernel(co
 #pragma unroll
     for (int j = 0; j < 4; ++j) sums[g][lane * 4 + j] = s[j];
     __syncthreads();
-    const long long c = (long long)blockIdx.x * 128 + threadIdx.x;
-    if (threadIdx.x < 128 && c < n) {
-        double t = sums[0][threadIdx.x];
+    const int c = threadIdx.x & 31, part = threadIdx.x >> 5;
+    if (part < kFoldGroups / 8) {
+        double t = sums[part * 8][c];
 #pragma unroll
-        for (int k = 1; k < kFoldGroups; ++k) t += sums[k][threadIdx.x];
-        gw[c] = (float)t;
+        for (int k = 1; k < 8; ++k) t += sums[part * 8 + k][c];
+        eights[part][c] = t;
+    }
+    __syncthreads();
+    if (part == 0 && (long long)blockIdx.x * 32 + c < n) {
+        double t = eights[0][c];
+#pragma unroll
+        for (int k = 1; k < kFoldGroups / 8; ++k) t += eights[k][c];
+        gw[(long long)blockIdx.x * 32 + c] = (float)t;
     }
 }
 
@@ -323,7 +330,10 @@ extern "C" ag_status_t ag_rms_norm_f32(ag_stream_t stream, const float *x, const
     if (cells <= 512) NORM(64, 2);
     else if (cells <= 1024) NORM(64, 4);
     else if (cells <= 2048) NORM(256, 2);
+    else if (cells <= 1024 * 3) NORM(256, 3);
     else if (cells <= 4096) NORM(256, 4);
+    else if (cells <= 5120) NORM(256, 5);
+    else if (cells <= 6144) NORM(256, 6);
     else if (cells <= 8192) NORM(256, 8);
     else if (cells <= 16384) NORM(1024, 4);
     else if (cells <= kMaxRegisterRow) NORM(1024, 8);
@@ -366,7 +376,9 @@ extern "C" ag_status_t ag_rms_norm_grad_f32(ag_stream_t stream, const float *h, 
     else if (n <= 512) GRAD(64, 2);
     else if (n <= kWaveRow) GRAD(64, 4);
     else if (n <= 2048) GRAD(256, 2);
+    else if (n <= 1024 * 3) GRAD(256, 3);
     else if (n <= 4096) GRAD(256, 4);
+    else if (n <= 6144) GRAD(512, 3);
     else if (n <= 8192) GRAD(512, 4);
     else if (n <= 16384) GRAD(1024, 4);
     else {
@@ -375,7 +387,7 @@ extern "C" ag_status_t ag_rms_norm_grad_f32(ag_stream_t stream, const float *h, 
     }
 #undef GRAD
     if (gw)
-        hipLaunchKernelGGL(rms_norm_grad_fold_kernel, dim3((unsigned)((n + 127) / 128)), dim3(kFoldGroups * 32), 0, st,
+        hipLaunchKernelGGL(rms_norm_grad_fold_kernel, dim3((unsigned)((n + 31) / 32)), dim3(kFoldGroups * 8), 0, st,
                            static_cast<const float *>(ws), gw, n, G);
     return check_launch("rms_norm_grad");
 }

@@ -58,6 +58,50 @@ def test_norm_is_the_formula_rounded_once(K, rng, rows, with_residual, n):
     assert torch.equal(h2, h) and torch.equal(rstd2, rstd)
 
 
+@pytest.mark.parametrize("n", [1, 2, 3, 5, 7, 253, 254, 257, 509, 1021, 1022, 1023, 2045, 2047, 4093, 4095, 5003, 8190, 16381, 16383])
+@pytest.mark.parametrize("places", [(0, 0, 0, 0), (1, 1, 1, 1), (3, 3, 3, 3), (2, 2, 2, 1), (0, 1, 2, 3)])
+def test_rows_and_arrays_that_start_anywhere_in_a_line(K, rng, places, n):
+    """Arrays whose first elements lie 0 to 3 elements behind a 16-byte boundary, alike or not: values, and nothing written
+    in front of or behind them."""
+    from rust_autograd_amd import capi
+    L = capi.lib()
+    rows = 13
+
+    def array(place, value=None):
+        buf = torch.full((rows * n + 16,), 7.0, device="cuda")
+        view = buf[4 + place:4 + place + rows * n].view(rows, n)
+        if value is not None:
+            view.copy_(value)
+        return buf, view
+
+    def untouched(buf, place):
+        return bool((buf[:4 + place] == 7.0).all()) and bool((buf[4 + place + rows * n:] == 7.0).all())
+
+    w = dev(1 + 0.2 * rng.standard_normal(n))
+    x, res, gy = (dev(sample(rng, rows, n)) for _ in range(3))
+    (_, vx), (_, vr), (bh, vh), (by, vy) = array(places[0], x), array(places[1], res), array(places[2]), array(places[3])
+    rstd = torch.empty(rows, device="cuda")
+    capi.check(L.ag_rms_norm_f32(K._stream(), vx.data_ptr(), vr.data_ptr(), w.data_ptr(), 1e-6, vh.data_ptr(), vy.data_ptr(), None, None,
+                                 rstd.data_ptr(), rows, n))
+    h32 = x.cpu().numpy() + res.cpu().numpy()
+    eps = float(np.float32(1e-6))
+    want, r = plain64.rms_norm(h32, host(w), eps)
+    assert np.array_equal(vh.cpu().numpy(), h32)
+    assert (np.abs(host(vy) - want) <= U * (1 + 1e-6) * np.abs(want) + TINY).all()
+    assert (np.abs(host(rstd) - r) <= U * (1 + 1e-6) * r).all()
+    assert untouched(bh, places[2]) and untouched(by, places[3])
+    (_, vg), (bx, vgx) = array(places[2], gy), array(places[3])
+    gw_buf = torch.full((n + 8,), 7.0, device="cuda")
+    nb = L.ag_rms_norm_grad_f32_workspace(rows, n)
+    ws = torch.full((nb // 4 + 8,), 7.0, device="cuda")
+    capi.check(L.ag_rms_norm_grad_f32(K._stream(), vh.data_ptr(), w.data_ptr(), rstd.data_ptr(), vg.data_ptr(), vx.data_ptr(), vgx.data_ptr(),
+                                      gw_buf[3:].data_ptr(), rows, n, ws.data_ptr(), nb))
+    want_x, want_w, size_x, size_w = plain64.rms_norm_grad(h32, host(w), eps, host(gy), host(x))
+    assert (np.abs(host(vgx) - want_x) <= 6 * U * size_x + TINY).all()
+    assert (np.abs(host(gw_buf[3:3 + n]) - want_w) <= (rows + 4) * U * size_w + TINY).all()
+    assert untouched(bx, places[3]) and (gw_buf[:3] == 7.0).all() and (gw_buf[3 + n:] == 7.0).all() and (ws[nb // 4:] == 7.0).all()
+
+
 def test_norm_of_many_rows_and_leading_axes(K, rng):
     x, w = sample(rng, 3000, 257), sample(rng, 1, 257)[0]
     y, _, _ = K.rms_norm(dev(x).view(30, 100, 257), dev(w), 1e-6)
