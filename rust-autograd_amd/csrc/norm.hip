@@ -69,10 +69,11 @@ __device__ inline void norm_write(const NormArgs &a, size_t row, long long i, qu
 // One row per T threads, held in registers (Q quads a thread: rows of up to 4 * Q * T elements), so every input is read
 // once; T = 64 packs four rows into a block of 256.  Behind the row's end quads are zero: they pad the 8-bit output.
 // Bound by HBM: 16384 x 8192 with residual and 8-bit output 270 us (6.4 TB/s; a copy of 4 GiB reaches 4.7; 16 us more
-// without streaming stores and loads, 15 with the half wave's maxima exchanged through LDS); one row of 4096 4.8 us.  Stores stream always (1024 x 4096: 9.7 and
-// 12.5 us), loads from kStreamBytes on, beyond what the last-level cache keeps between two kernels (4096 x 4096, whose
-// arrays it does keep: 36 us without, 39 with; 16384 x 4096: 151 and 139).  The quads of a thread come in small steps of
-// the row's length: 16384 x 5001 to 8 bits 202 us with 5 quads a thread, 233 with 8; its gradient 251 and 336.
+// without streaming stores and loads, 15 with the half wave's maxima exchanged through LDS); one row of 4096 4.8 us.
+// Stores stream always (1024 x 4096: 9.7 and 12.5 us), loads from kStreamBytes on, beyond what the last-level cache keeps
+// between two kernels (4096 x 4096, whose arrays it does keep: 36 us without, 39 with; 16384 x 4096: 151 and 139).  The
+// quads of a thread come in small steps of the row's length: 16384 x 5001 to 8 bits 202 us with 5 quads a thread, 233
+// with 8; its gradient 251 and 336.
 template <int T, int Q, bool STREAM>
 __global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_kernel(NormArgs a, unsigned rows)
 {
@@ -330,7 +331,7 @@ extern "C" ag_status_t ag_rms_norm_f32(ag_stream_t stream, const float *x, const
     if (cells <= 512) NORM(64, 2);
     else if (cells <= 1024) NORM(64, 4);
     else if (cells <= 2048) NORM(256, 2);
-    else if (cells <= 1024 * 3) NORM(256, 3);
+    else if (cells <= 2560) NORM(128, 5);
     else if (cells <= 4096) NORM(256, 4);
     else if (cells <= 5120) NORM(256, 5);
     else if (cells <= 6144) NORM(256, 6);
@@ -376,7 +377,6 @@ extern "C" ag_status_t ag_rms_norm_grad_f32(ag_stream_t stream, const float *h, 
     else if (n <= 512) GRAD(64, 2);
     else if (n <= kWaveRow) GRAD(64, 4);
     else if (n <= 2048) GRAD(256, 2);
-    else if (n <= 1024 * 3) GRAD(256, 3);
     else if (n <= 4096) GRAD(256, 4);
     else if (n <= 6144) GRAD(512, 3);
     else if (n <= 8192) GRAD(512, 4);

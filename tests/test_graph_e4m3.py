@@ -90,6 +90,26 @@ def test_product_and_gradients_of_integers_are_exact(G, rng, m, k, n, ta, tb):
 
 
 @pytest.mark.gpu
+def test_second_order_and_a_tensor_against_itself(G, rng):
+    """Integers, exact: d/dw of sum(v * d/dx sum(g * x w)) is the product of v and g; the gradient of x x^T has both of x's
+    shares, and its two operands are one rounding."""
+    env, c = context(G)
+    m, k, n = 40, 150, 33
+    x, w, g, v = (rng.integers(-2, 3, s) for s in ((m, k), (k, n), (m, n), (m, k)))
+    xt, wt = c.placeholder("x", [m, k]), c.placeholder("w", [k, n])
+    gt, vt = c.placeholder("g", [m, n]), c.placeholder("v", [m, k])
+    gx = c.grad_with_default([c.matmul_e4m3(xt, wt)], [xt], [gt])[0]
+    second = c.grad([c.mul(gx, vt)], [wt, gt])
+    square = c.matmul_e4m3(xt, xt, False, True)
+    st = c.placeholder("s", [m, m])
+    s = rng.integers(-2, 3, (m, m))
+    gsq = c.grad_with_default([square], [xt], [st])[0]
+    dw, dg, sq, gs = c.eval([*second, square, gsq], {"x": x, "w": w, "g": g, "v": v, "s": s})
+    assert np.array_equal(dw, v.T @ g) and np.array_equal(dg, v @ w)
+    assert np.array_equal(sq, x @ x.T) and np.array_equal(gs, (s + s.T) @ x)
+
+
+@pytest.mark.gpu
 def test_product_of_rounded_operands(G, rng):
     env, c = context(G)
     m, k, n = 70, 400, 200
