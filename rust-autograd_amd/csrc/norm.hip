@@ -93,8 +93,12 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_kernel(NormArgs a,
 #pragma unroll
         for (int k = 0; k < Q; ++k) h[k] += b[k];
     }
+    // The weight stays in cache.  It is read ahead of the sum, so that one row alone does not wait twice (1 x 8192 4.9 us,
+    // behind it 5.7), but for the longest rows, whose registers it would spill (2048 x 32768 199 us, ahead 271).
+    constexpr bool LATE = T == 1024 && Q == 8;
+    if (!LATE)
 #pragma unroll
-    for (int k = 0; k < Q; ++k) w[k] = load_quad(a.weight, (long long)(k * T + t) * 4, a.n);
+        for (int k = 0; k < Q; ++k) w[k] = load_quad(a.weight, (long long)(k * T + t) * 4, a.n);
     double s = 0.0;
 #pragma unroll
     for (int k = 0; k < Q; ++k) s = square_sum(h[k], s);
@@ -105,6 +109,7 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_kernel(NormArgs a,
     for (int k = 0; k < Q; ++k) {
         const long long i = (long long)(k * T + t) * 4;
         if (a.h) store_quad<true>(a.h + row * a.n, i, a.n, h[k]);
+        if (LATE) w[k] = load_quad(a.weight, i, a.n);
         norm_write(a, row, i, norm_quad(h[k], w[k], r));
     }
 }
@@ -337,6 +342,7 @@ extern "C" ag_status_t ag_rms_norm_f32(ag_stream_t stream, const float *x, const
     else if (cells <= 6144) NORM(256, 6);
     else if (cells <= 8192) NORM(256, 8);
     else if (cells <= 16384) NORM(1024, 4);
+    else if (cells <= 20480) NORM(1024, 5);
     else if (cells <= kMaxRegisterRow) NORM(1024, 8);
     else hipLaunchKernelGGL(rms_norm_long_kernel, dim3(R), dim3(kLongT), 0, st, a);
 #undef NORM
