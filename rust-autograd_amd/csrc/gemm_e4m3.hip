@@ -60,8 +60,8 @@ __device__ inline const unsigned char *uniform(const unsigned char *p)
     return reinterpret_cast<const unsigned char *>(((unsigned long long)hi << 32) | lo);
 }
 
-// BM x BN of C per block, WM x WN per wave, 128 of the contraction per step.  LDS holds two steps of both operands, rows of
-// 128 bytes, and a word of scales per row (four blocks, one of which the step uses).  The 16-byte piece c of row r stands
+// BM x BN of C per block, WM x WN per wave, 128 of the contraction per step.  LDS holds STAGES steps of both operands, rows
+// of 128 bytes, and a word of scales per row (four blocks, one of which the step uses).  The 16-byte piece c of row r stands
 // at place c ^ (r & 7) ^ ((r >> 3) & 1), so that 16 consecutive rows read at one piece fall on all 64 banks.
 //
 // What bounds it is power: with Gaussian operands the chip holds the matrix instruction alone, fed from registers, at
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void gemm_e4m3_tile_kerne
 {
     constexpr int WAVES_N = BN / WN, NW = BM / WM * WAVES_N, MI = WM / 32, NI = WN / 32;
     constexpr int ROWS = BM + BN, STEP = ROWS * 128;
-    constexpr int LOADS = ROWS / 8 / NW;         // 1 KiB loads (8 rows) of a wave per step
+    constexpr int LOADS = ROWS / 8 / NW;                    // 1 KiB loads (8 rows) of a wave per step
     constexpr int SCALE_LOADS = (ROWS / 64 + NW - 1) / NW;  // 64 words of a wave per step
     static_assert(STAGES >= 2 && STAGES <= 4, "ring of two to four steps");
     static_assert(ROWS % (8 * NW) == 0 && BM % 64 == 0 && BN % 64 == 0, "rows divide over the waves");
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void gemm_e4m3_tile_kerne
         const int first = in_a ? m0 + r0 : n0 + r0 - BM, last = (in_a ? p.M : p.N) - 1;
         const int start = min(first, last), row = min(first + (lane >> 3), last);
         base[i] = uniform((in_a ? p.a : p.b) + start * p.pitch);
-        // (a row's pitch is at most 2^31: 8 rows pass 32 bits only where one row is longer than 2^28, which the host refuses)
+        // (rows are at most 2^28 bytes long, which the host checks: 8 of them stay within 32 bits)
         offset[i] = (unsigned)((row - start) * p.pitch) + (unsigned)(((lane & 7) ^ (lane >> 3) ^ ((i * NW + wave) & 1)) * 16);
     }
     const unsigned char *scale_base[SCALE_LOADS];
@@ -290,6 +290,13 @@ __global__ __launch_bounds__(256) void gemm_e4m3_fold_kernel(const float *__rest
 // layout that hold them 12.0 and 32 us.  At 4 rows the two ways are even (10.0 and 10.2, 22.8 and 20.8 us).
 constexpr int kRoundedRows = 4;
 
+// Between LDS accesses of lanes of one wave: they complete in their order, which the compiler must not change.
+__device__ inline void hand_over()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 template <int MT, int NW, int XR>
 __global__ __launch_bounds__(NW * 64) void gemm_e4m3_skinny_kernel(GemmE4m3 p, const float *__restrict__ x, long long ldx, int K)
 {
@@ -357,7 +364,7 @@ __global__ __launch_bounds__(NW * 64) void gemm_e4m3_skinny_kernel(GemmE4m3 p, c
             if (p.M == 1) round_rows(std::integral_constant<int, 1>());
             else if (p.M == 2) round_rows(std::integral_constant<int, 2>());
             else round_rows(std::integral_constant<int, 4>());
-            __builtin_amdgcn_wave_barrier();  // (only this wave reads them: its LDS accesses complete in order)
+            hand_over();
             const bool here = r16 < p.M;
             word_a[0] = here ? *reinterpret_cast<const unsigned *>(rounded_scales[wave][here ? r16 : 0]) : 0x7f7f7f7fu;
 #pragma unroll
@@ -367,7 +374,7 @@ __global__ __launch_bounds__(NW * 64) void gemm_e4m3_skinny_kernel(GemmE4m3 p, c
                     const v4i q = *reinterpret_cast<const v4i *>(&rounded[wave][here ? r16 : 0][u * 128 + group * 32 + h * 16]);
                     qa[0][u][h] = here ? q : v4i{0, 0, 0, 0};
                 }
-            __builtin_amdgcn_wave_barrier();
+            hand_over();
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u)
