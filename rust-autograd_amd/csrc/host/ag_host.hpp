@@ -233,6 +233,10 @@ class Op {
     virtual const char *name() const = 0;
     virtual OpError compute(ComputeContext &ctx) const = 0;
     virtual void grad(GradientContext &ctx) const = 0;
+    // The node is no step of the program but another form of its input, which the nodes that read it share: they see the
+    // input as it is at their own turn.  The evaluator computes such a node again for a reader behind an in-place update
+    // of a variable that the node reads.
+    virtual bool is_form_of_input() const { return false; }
     // Evaluation-time fusion with the op that produces input 0 (no counterpart in the reference, whose evaluator
     // runs every node on its own, src/evaluation.rs:310-329).  When the evaluator reaches a node whose first input has
     // not been computed yet and fuses_with_producer(that input's op) holds, it gathers the PRODUCER's inputs and behind

@@ -1432,6 +1432,7 @@ struct QuantizeE4m3 : Op {
     int orientation;
     explicit QuantizeE4m3(int o) : orientation(o) {}
     const char *name() const override { return "QuantizeE4m3"; }
+    bool is_form_of_input() const override { return true; }
     OpError compute(ComputeContext &ctx) const override
     {
         const NdArray x = ctx.input(0);

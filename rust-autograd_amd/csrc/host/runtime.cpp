@@ -666,6 +666,12 @@ namespace {
 struct StorageEntry {
     OpError error;
     std::vector<NdArray> outputs;
+    // The variables that a form of them (Op::is_form_of_input) was computed from, as they were then.
+    std::vector<std::pair<NdArray, int64_t>> variables;
+    bool outdated() const
+    {
+        return std::any_of(variables.begin(), variables.end(), [](const auto &v) { return v.first.version() != v.second; });
+    }
 };
 
 const NdArray *find_placeholder(const std::vector<std::pair<std::string, NdArray>> &feeds, const TensorInternal &n)
@@ -770,13 +776,16 @@ std::vector<EvalResult> Context::eval(const std::vector<Tensor> &tensors,
                 return;
             }
     };
-    // Runs one node the ordinary way and files its result.
-    auto run_node = [&](const TensorInternal &n) {
+    // Runs one node, whose inputs are all there, and files its result.
+    auto run_one = [&](const TensorInternal &n) {
         std::vector<ComputeContext::Input> inputs;
         OpError status = gather(n, &inputs);
         StorageEntry entry;
         if (status.ok()) {
             flush_if_touched(inputs);
+            if (n.op->is_form_of_input())
+                for (const ComputeContext::Input &x : inputs)
+                    if (x.kind != ComputeContext::InputKind::NonVariable) entry.variables.emplace_back(x.array, x.array.version());
             ComputeContext cc(std::move(inputs), &deferred);
             status = n.op->compute(cc);
             if (status.ok()) {
@@ -786,7 +795,13 @@ std::vector<EvalResult> Context::eval(const std::vector<Tensor> &tensors,
             if (trace_enabled()) trace_node(n, entry.outputs, status);
         }
         entry.error = status;
-        storage.emplace(n.id, std::move(entry));
+        storage[n.id] = std::move(entry);
+    };
+    // The same behind the forms among its inputs whose variables have been updated since, which are computed again.
+    auto run_node = [&](const TensorInternal &n) {
+        for (const IncomingTensor &in : n.incoming_nodes)
+            if (auto it = storage.find(in.id); it != storage.end() && it->second.outdated()) run_one(node(in.id));
+        run_one(n);
     };
     // The producer of a node's first input when the two can be evaluated in one pass (Op::fuses_with_producer).
     auto fusable_producer = [&](const TensorInternal &n) -> const TensorInternal * {

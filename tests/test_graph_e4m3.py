@@ -245,3 +245,62 @@ def test_a_quantised_network_trains_with_clipped_adam(G, rng):
     for p, q, s in zip(a, b, start.values()):
         assert np.isfinite(p).all() and not np.array_equal(p, s.astype(np.float32))
         assert np.array_equal(p, q)
+
+
+# ---- weights that change within an evaluation (tensors are visited from the last to the first) ---------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["behind", "in front", "both sides"])
+@pytest.mark.parametrize("kind,ta,tb", [("matmul", False, False), ("matmul_e4m3", False, False), ("matmul_e4m3", False, True), ("matmul_e4m3", True, False)])
+def test_a_product_reads_the_weight_as_it_is_at_its_turn(G, rng, kind, order, ta, tb):
+    """The weight is trained by an update of the same evaluation, whose gradients share the products' operands: a product
+    behind the update has the bits of one of the updated weight, a product in front of it those of the old one."""
+    k, n = 200, 72
+    env = G.VariableEnvironment()
+    w = env.set("w", rng.standard_normal((n, k) if tb else (k, n)))
+    adam = G.Adam(env, [w], alpha=0.5)
+    feeds = {"x": rng.standard_normal((k, 24) if ta else (24, k)), "z": rng.standard_normal((k, 40) if ta else (40, k))}
+
+    def product(c, name):
+        x = c.placeholder(name, list(feeds[name].shape))
+        return c.matmul(x, c.variable(w)) if kind == "matmul" else c.matmul_e4m3(x, c.variable(w), ta, tb)
+
+    def alone():  # of the weight as it is now
+        c = env.context()
+        return c.eval([product(c, "z")], feeds)[0]
+
+    old = alone()
+    c = env.context()
+    y, wt = product(c, "x"), c.variable(w)
+    update = adam.get_update_op([wt], c.grad([c.sum_all(c.mul(y, y))], [wt]), c)
+    if order == "behind":
+        after, before = c.eval([product(c, "z"), update], feeds)[0], None
+    elif order == "in front":
+        after, before = None, c.eval([update, product(c, "z")], feeds)[1]
+    else:
+        after, _, before = c.eval([product(c, "z"), update, product(c, "z")], feeds)
+    new = alone()
+    assert not np.array_equal(old, new)
+    assert after is None or np.array_equal(after, new)
+    assert before is None or np.array_equal(before, old)
+
+
+@pytest.mark.gpu
+def test_both_operands_and_several_updates(G, rng):
+    """x x^T of a variable on both sides, between and behind two updates of it."""
+    env = G.VariableEnvironment()
+    x = env.set("x", rng.standard_normal((30, 140)))
+    adam = G.Adam(env, [x], alpha=0.25)
+    c = env.context()
+    xt = c.variable(x)
+
+    def square(c):
+        return c.matmul_e4m3(c.variable(x), c.variable(x), False, True)
+
+    def update(g):
+        return adam.get_update_op([xt], [c.placeholder(g, [30, 140])], c)
+
+    feeds = {"g": rng.standard_normal((30, 140)), "h": rng.standard_normal((30, 140))}
+    third, _, second, _, first = c.eval([square(c), update("h"), square(c), update("g"), square(c)], feeds)
+    c = env.context()
+    assert np.array_equal(third, c.eval([square(c)])[0])
+    assert not np.array_equal(first, second) and not np.array_equal(second, third)
