@@ -240,7 +240,8 @@ class Op {
     // Evaluation-time fusion with the op that produces input 0 (no counterpart in the reference, whose evaluator
     // runs every node on its own, src/evaluation.rs:310-329).  When the evaluator reaches a node whose first input has
     // not been computed yet and fuses_with_producer(that input's op) holds, it gathers the PRODUCER's inputs and behind
-    // them the node's own from the second on (which have to be variables or placeholders), and calls
+    // them the node's own from the second on (which have to be variables or placeholders; where a variable among them is
+    // updated before the node's own turn, the node is computed again then, by itself), and calls
     // compute_with_producer: the op may then write the producer's outputs (`producer_outputs`) and its own
     // (ctx) in one pass and return true, or touch nothing and return false, upon which both nodes are evaluated the
     // ordinary way.  The results must have the bits of the two nodes evaluated in turn.

@@ -8,6 +8,7 @@
 #include <cstring>
 #include <mutex>
 #include <stdexcept>
+#include <unordered_set>
 
 #include "ag_hip.h"
 #include "ag_host.hpp"
@@ -666,8 +667,16 @@ namespace {
 struct StorageEntry {
     OpError error;
     std::vector<NdArray> outputs;
-    // The variables that a form of them (Op::is_form_of_input) was computed from, as they were then.
+    // Computed ahead of its turn, along with its producer, which was asked for first: not read before its turn comes.
+    bool ahead = false;
+    // The variables that this may have to be computed again for, as they were: those that a form (Op::is_form_of_input) was
+    // computed from, and those that a node computed ahead of its turn read.
     std::vector<std::pair<NdArray, int64_t>> variables;
+    void note_variables(const std::vector<ComputeContext::Input> &inputs, size_t first)
+    {
+        for (size_t i = first; i < inputs.size(); ++i)
+            if (inputs[i].kind != ComputeContext::InputKind::NonVariable) variables.emplace_back(inputs[i].array, inputs[i].array.version());
+    }
     bool outdated() const
     {
         return std::any_of(variables.begin(), variables.end(), [](const auto &v) { return v.first.version() != v.second; });
@@ -736,7 +745,9 @@ std::vector<EvalResult> Context::eval(const std::vector<Tensor> &tensors,
         }
     } flush_on_unwind{deferred};
     auto would_not_visit = [&](const TensorInternal &n) {
-        return n.is_placeholder || n.is_variable() || storage.count(n.id) != 0;
+        if (n.is_placeholder || n.is_variable()) return true;
+        const auto it = storage.find(n.id);
+        return it != storage.end() && !it->second.ahead;
     };
     std::vector<std::pair<TensorID, bool>> dfs;
     for (const Tensor &t : tensors) {
@@ -783,9 +794,7 @@ std::vector<EvalResult> Context::eval(const std::vector<Tensor> &tensors,
         StorageEntry entry;
         if (status.ok()) {
             flush_if_touched(inputs);
-            if (n.op->is_form_of_input())
-                for (const ComputeContext::Input &x : inputs)
-                    if (x.kind != ComputeContext::InputKind::NonVariable) entry.variables.emplace_back(x.array, x.array.version());
+            if (n.op->is_form_of_input()) entry.note_variables(inputs, 0);
             ComputeContext cc(std::move(inputs), &deferred);
             status = n.op->compute(cc);
             if (status.ok()) {
@@ -819,8 +828,11 @@ std::vector<EvalResult> Context::eval(const std::vector<Tensor> &tensors,
         return &p;
     };
     // Which of the nodes this evaluation will reach are such producers, and of which node: whoever asks for the
-    // producer first is sent to that node instead, so the pair runs fused whatever the order of the walk.
+    // producer first is sent to that node instead, so the pair runs fused whatever the order of the walk.  The node may
+    // then run ahead of its turn, and a variable that it reads beside the producer's inputs be updated in between: when
+    // its turn comes and one was, it is computed again, from the producer's output.
     std::unordered_map<TensorID, TensorID> fused_into;
+    std::unordered_set<TensorID> sent_to;
     {
         std::vector<TensorID> stack;
         std::unordered_map<TensorID, bool> seen;
@@ -843,11 +855,19 @@ std::vector<EvalResult> Context::eval(const std::vector<Tensor> &tensors,
         if (!should_visit) {
             if (auto it = fused_into.find(id); it != fused_into.end() && !would_not_visit(n) && storage.count(it->second) == 0) {
                 dfs.emplace_back(it->second, false);  // the node that computes this one along with itself
+                sent_to.insert(it->second);
                 continue;
             }
         }
         if (should_visit) {
             if (would_not_visit(n)) continue;
+            if (auto it = storage.find(id); it != storage.end()) {  // computed ahead of its turn, which is now
+                const bool outdated = it->second.outdated();
+                it->second.ahead = false;
+                it->second.variables.clear();
+                if (outdated) run_node(n);
+                continue;
+            }
             if (const TensorInternal *p = fusable_producer(n); p && storage.count(p->id) == 0) {
                 // the producer has not run: both nodes in one pass, from the producer's inputs (which the first visit
                 // below has put in front of this node)
@@ -857,8 +877,10 @@ std::vector<EvalResult> Context::eval(const std::vector<Tensor> &tensors,
                 bool fused = false;
                 if (status.ok()) {
                     flush_if_touched(inputs);
-                    ComputeContext cc(std::move(inputs), &deferred);
                     StorageEntry pe, ne;
+                    if (sent_to.count(id)) ne.note_variables(inputs, p->incoming_nodes.size());
+                    ne.ahead = !ne.variables.empty();
+                    ComputeContext cc(std::move(inputs), &deferred);
                     fused = n.op->compute_with_producer(cc, *p->op, &pe.outputs, &status);
                     if (fused) {
                         ++fused_pairs_;
@@ -879,6 +901,7 @@ std::vector<EvalResult> Context::eval(const std::vector<Tensor> &tensors,
                 }
                 if (fused) continue;
                 run_node(*p);  // not this time (extents the fused form does not take, or an input in error)
+                if (sent_to.count(id)) continue;  // (only the producer has been asked for so far)
             }
             run_node(n);
         } else {

@@ -304,3 +304,55 @@ def test_both_operands_and_several_updates(G, rng):
     c = env.context()
     assert np.array_equal(third, c.eval([square(c)])[0])
     assert not np.array_equal(first, second) and not np.array_equal(second, third)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["sum first", "norm first", "sum behind"])
+def test_a_norm_reads_its_weight_as_it_is_at_its_turn(G, rng, order):
+    """A sum and the norm behind it, with an update of the norm's weight between them that does not wait for the norm: with
+    and without the pass over both the norm takes the weight of its own turn, and so does a product that reads it."""
+    a, b, w = (rng.standard_normal(s) for s in ((50, 260), (50, 260), (260,)))
+    proj = rng.standard_normal((260, 40)) / 16
+
+    def run():
+        env = G.VariableEnvironment()
+        wid, pid = env.set("w", w), env.set("proj", proj)
+        adam = G.Adam(env, [wid], alpha=0.5)
+        c = env.context()
+        h = c.placeholder("a", [50, 260]) + c.placeholder("b", [50, 260])
+        y = c.rms_norm(h, c.variable(wid))
+        z = c.matmul_e4m3(y, c.variable(pid))
+        update = adam.get_update_op([c.variable(wid)], [c.placeholder("g", [260])], c)
+        ts = {"sum first": [z, y, update, h], "norm first": [h, update, z, y], "sum behind": [h, z, y, update]}[order]
+        got = dict(zip((t.id for t in ts), c.eval(ts, {"a": a, "b": b, "g": np.ones(260)})))
+        return [got[t.id] for t in (h, y, z)], env.array(wid)
+
+    try:
+        (h, y, z), new = run()
+        G.set_shortcuts(False)
+        plain, same = run()
+    finally:
+        G.set_shortcuts(True)
+    assert np.array_equal(new, same) and not np.array_equal(new, w.astype(np.float32))
+    for p, q in zip((h, y, z), plain):
+        assert np.array_equal(p, q)
+    weight = w.astype(np.float32) if order == "norm first" else new
+    want = plain64.rms_norm(h, weight, float(np.float32(1e-6)))[0]
+    assert (np.abs(y - want) <= U * (1 + 1e-6) * np.abs(want)).all()
+
+
+@pytest.mark.gpu
+def test_a_norm_keeps_the_pass_of_the_sum_where_its_weight_is_trained_behind_it(G, rng):
+    """The sum is asked for first and the update of the norm's weight waits for the norm, as in a training step."""
+    env = G.VariableEnvironment()
+    w = env.set("w", 1 + 0.1 * rng.standard_normal(130))
+    adam = G.Adam(env, [w], alpha=0.5)
+    c = env.context()
+    h = c.placeholder("a", [20, 130]) + c.placeholder("b", [20, 130])
+    y = c.rms_norm(h, c.variable(w))
+    update = adam.get_update_op([c.variable(w)], c.grad([c.sum_all(c.mul(y, y))], [c.variable(w)]), c)
+    a, b, old = rng.standard_normal((20, 130)).astype(np.float32), rng.standard_normal((20, 130)).astype(np.float32), env.array(w)
+    yv, _, hv = c.eval([y, update, h], {"a": a, "b": b})
+    assert c.fused_pairs == 1 and np.array_equal(hv, a + b) and not np.array_equal(env.array(w), old)
+    want = plain64.rms_norm(hv, old, float(np.float32(1e-6)))[0]
+    assert (np.abs(yv - want) <= U * (1 + 1e-6) * np.abs(want)).all()
