@@ -419,9 +419,10 @@ ag_status_t ag_rms_norm_f32(ag_stream_t stream, const float *x, const float *res
                             float *h, float *y, uint8_t *q, uint8_t *scales, float *rstd, int rows, int n);
 
 /* Its gradient: gx = rstd * weight * gy - h * rstd^3 / n * sum(weight * gy * h) (+ gh, the gradient that reaches h on
- * other ways; may be NULL), which is that of x and of residual, and gw [n] = sum over rows of gy * h * rstd, added in an
- * order that depends on the extents only.  gx or gw may be NULL; gx may be the array gy or gh.  ws (for gw):
- * ag_rms_norm_grad_f32_workspace() bytes. */
+ * other ways; may be NULL), which is that of x and of residual, in 64 bits and rounded to f32 once, and gw [n] = sum over
+ * rows of gy * h * rstd, added in an order that depends on the extents only.  (rstd is what the f32 array holds: infinite
+ * for rows of a root mean square below 2^-128 with eps 0, of fewer digits above 2^126.)  gx or gw may be NULL; gx may be
+ * the array gy or gh.  ws (for gw): ag_rms_norm_grad_f32_workspace() bytes. */
 size_t ag_rms_norm_grad_f32_workspace(int rows, int n);
 ag_status_t ag_rms_norm_grad_f32(ag_stream_t stream, const float *h, const float *weight, const float *rstd,
                                  const float *gy, const float *gh, float *gx, float *gw, int rows, int n, void *ws,

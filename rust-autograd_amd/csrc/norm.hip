@@ -156,11 +156,13 @@ __device__ inline double dot3(quad_t g, quad_t w, quad_t h, double s)
     for (int j = 0; j < 4; ++j) s = fma((double)g[j] * (double)w[j], (double)h[j], s);
     return s;
 }
-__device__ inline quad_t grad_quad(quad_t h, quad_t w, quad_t g, float r, float c)
+// r w gy - h c + gh, c = sum(w gy h) / n * r^3, rounded to f32 once.  In 64 bits: c is about w gy / h^2 and leaves f32's
+// range where the gradient does not (h of 1e20 and gy of 1e-3: c = 1e-43), and so may w gy.
+__device__ inline quad_t grad_quad(quad_t h, quad_t w, quad_t g, quad_t gh, double r, double c)
 {
     quad_t o;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = fmaf(-h[j], c, g[j] * w[j] * r);
+    for (int j = 0; j < 4; ++j) o[j] = (float)fma(-(double)h[j], c, fma((double)g[j] * (double)w[j], r, (double)gh[j]));
     return o;
 }
 
@@ -195,14 +197,20 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_grad_kernel(NormGr
 #pragma unroll
         for (int k = 0; k < Q; ++k) s = dot3(g[k], w[k], h[k], s);
         s = block_sum<T>(s, part[turn]);  // (two arrays in turn: the next row's sums do not wait for this row's readers)
-        const float c = (float)(s / (double)a.n * (double)r * (double)r * (double)r);
+        const double c = s / (double)a.n * (double)r * (double)r * (double)r;
 #pragma unroll
         for (int k = 0; k < Q; ++k) {
             const long long i = (long long)(k * T + t) * 4;
+            // The row stays in f32 over the sum; left to itself the compiler keeps what dot3 widened, in twice the registers
+            // (2048 x 16384 114 us, widened 174).  Short rows have some to spare, for the weight (200000 x 128 57 us, all in
+            // f32 61, all widened 79) or the products (65536 x 512 103, all in f32 106).
+            if (T == 64 && Q == 1) asm volatile("" : "+v"(h[k]), "+v"(g[k]));
+            else if (T == 64 && Q == 2) asm volatile("" : "+v"(h[k]));
+            else asm volatile("" : "+v"(h[k]), "+v"(g[k]), "+v"(w[k]));
             if (a.gx) {
-                quad_t o = grad_quad(h[k], w[k], g[k], r, c);
-                if (a.gh) o += load_quad<STREAM>(a.gh + row * a.n, i, a.n);
-                store_quad<true>(a.gx + row * a.n, i, a.n, o);
+                quad_t gh = {0.f, 0.f, 0.f, 0.f};
+                if (a.gh) gh = load_quad<STREAM>(a.gh + row * a.n, i, a.n);
+                store_quad<true>(a.gx + row * a.n, i, a.n, grad_quad(h[k], w[k], g[k], gh, r, c));
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[k][j] = fmaf(g[k][j], h[k][j] * r, acc[k][j]);
@@ -246,11 +254,11 @@ __global__ __launch_bounds__(kLongT) void rms_norm_grad_long_kernel(NormGradArgs
         s = dot3(load_quad(gr, i, a.n), load_quad(a.weight, i, a.n), load_quad(hr, i, a.n), s);
     s = block_sum<kLongT>(s, part);
     const float r = a.rstd[row];
-    const float c = (float)(s / (double)a.n * (double)r * (double)r * (double)r);
+    const double c = s / (double)a.n * (double)r * (double)r * (double)r;
     for (long long i = (long long)threadIdx.x * 4; i < a.n; i += kLongT * 4) {
-        quad_t o = grad_quad(load_quad(hr, i, a.n), load_quad(a.weight, i, a.n), load_quad(gr, i, a.n), r, c);
-        if (a.gh) o += load_quad(a.gh + row * a.n, i, a.n);
-        store_quad(a.gx + row * a.n, i, a.n, o);
+        quad_t gh = {0.f, 0.f, 0.f, 0.f};
+        if (a.gh) gh = load_quad(a.gh + row * a.n, i, a.n);
+        store_quad(a.gx + row * a.n, i, a.n, grad_quad(load_quad(hr, i, a.n), load_quad(a.weight, i, a.n), load_quad(gr, i, a.n), gh, r, c));
     }
 }
 

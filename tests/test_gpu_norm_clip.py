@@ -204,6 +204,29 @@ def test_norm_gradient_against_differences(K, rng):
         assert abs((f(h64, w64 + d) - f(h64, w64 - d)) / (2 * step) - gw[j]) < 1e-6 * (1 + abs(gw[j]))
 
 
+@pytest.mark.parametrize("n", [3, 200, 1025, 4096, 8192, 16000, 20000, 40001])
+@pytest.mark.parametrize("gy_size,w_size", [(1.0, 1.0), (1e-3, 1.0), (1e-19, 1e-24), (1e18, 1e22)])
+def test_norm_gradient_over_the_range_of_f32(K, rng, gy_size, w_size, n):
+    """Rows whose squares, and products of gradient and weight, lie beyond f32's range while the gradient does not: the
+    roundings are counted as for any other rows."""
+    sizes = [h for h in (1e-36, 1e-30, 1e-20, 1.0, 1e18, 1e19, 1e20, 1e23, 1e30, 1e37) if 1e-36 <= gy_size * w_size / h <= 1e35]
+    rows = len(sizes)
+    assert rows >= 3
+    h, gy, gh = (rng.standard_normal((rows, n)) for _ in range(3))
+    h = (h * np.array(sizes)[:, None]).astype(np.float32)
+    gy = (gy * gy_size).astype(np.float32)
+    gh = (gh * (gy_size * w_size / np.array(sizes))[:, None]).astype(np.float32)
+    w = (rng.standard_normal(n) * w_size).astype(np.float32)
+    _, _, rstd = K.rms_norm(dev(h), dev(w), 0.0)
+    for other in (None, gh):
+        gx, gw = K.rms_norm_grad(dev(h), dev(w), rstd, dev(gy), gh=None if other is None else dev(other))
+        want_x, want_w, size_x, size_w = plain64.rms_norm_grad(h, w, 0.0, gy, other)
+        ex, ew = np.abs(host(gx) - want_x), np.abs(host(gw) - want_w)
+        say("gx error in u of its terms, by row: " + " ".join("%.2g" % v for v in (ex / size_x).max(1) / U))
+        assert (ex <= 6 * U * size_x + TINY).all()
+        assert (ew <= (rows + 4) * U * size_w + TINY).all()
+
+
 def test_norm_gradient_without_rows(K):
     z = torch.zeros
     gx, gw = K.rms_norm_grad(z(0, 8, device="cuda"), z(8, device="cuda"), z(0, device="cuda"), z(0, 8, device="cuda"))
