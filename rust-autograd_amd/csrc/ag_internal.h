@@ -24,8 +24,10 @@ inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 constexpr int kWave = 64;  // CDNA wavefront width
 
-// Largest grid.x HIP accepts.
-constexpr long long kMaxGridX = 2147483647LL;
+// HIP counts the threads of a grid along each axis in 32 bits: a launch of more runs what is left of their number modulo
+// 2^32, mostly without an error.
+constexpr long long kMaxThreadsX = 0xffffffffLL;
+constexpr long long kMaxGridX = kMaxThreadsX / 256;  // blocks of 256 threads
 
 constexpr int kXcds = 8;
 

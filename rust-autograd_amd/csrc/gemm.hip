@@ -871,7 +871,7 @@ static ag_status_t run_gemm(hipStream_t st, const char *who, const GemmCall &c, 
     p.tiles_m = (int)cdiv(c.M, kCfgs[cfg].bm);
     p.tiles_n = (int)cdiv(p.N, kCfgs[cfg].bn);
     const long long blocks = (long long)p.tiles_m * p.tiles_n * (fold ? 1 : c.batch) * p.splits;
-    AG_REQUIRE(blocks <= kMaxGridX, AG_ERR_INVALID_DIMS, "%s: too many tiles (%lld)", who, blocks);
+    AG_REQUIRE(blocks <= 0x7fffffffLL, AG_ERR_INVALID_DIMS, "%s: too many tiles (%lld)", who, blocks);
     p.total_blocks = (unsigned)blocks;
 
     // A persistent grid of G blocks takes ceil(items / G) rounds; when the last round would be
@@ -1008,7 +1008,7 @@ static ag_status_t conv_implicit_gemm(hipStream_t st, const float *wr, const flo
     p.tiles_m = (int)cdiv(C, kCfgs[cfg].bm);
     p.tiles_n = (int)cdiv(p.N, kCfgs[cfg].bn);
     const long long blocks = (long long)p.tiles_m * p.tiles_n;
-    AG_REQUIRE(blocks * p.splits <= kMaxGridX, AG_ERR_INVALID_DIMS, "conv2d_transpose: too many tiles (%lld)", blocks);
+    AG_REQUIRE(blocks * p.splits <= 0x7fffffffLL, AG_ERR_INVALID_DIMS, "conv2d_transpose: too many tiles (%lld)", blocks);
     p.total_blocks = (unsigned)(blocks * p.splits);
     // whole rounds of the persistent grid with the wide tile, then the remaining columns with a
     // narrower one (as for the folded GEMM over columns)

@@ -579,11 +579,16 @@ static bool plan_stream(const int *shape, int rank, const int *sorted_axes, int 
     return true;
 }
 
+// Lanes that launch_fold_rows gives to a row.
+static int fold_rows_lanes(size_t len, bool vec)
+{
+    const size_t lanes = vec ? len / 4 : len;
+    return lanes >= 32 ? 64 : lanes >= 8 ? 16 : 4;
+}
 static void launch_fold_rows(hipStream_t st, const float *src, float *dst, size_t rows, size_t len, float scale, int sc)
 {
     const bool vec = len % 4 == 0 && aligned16(src);
-    const size_t lanes = vec ? len / 4 : len;
-    const int G = lanes >= 32 ? 64 : lanes >= 8 ? 16 : 4;
+    const int G = fold_rows_lanes(len, vec);
     const dim3 grid((unsigned)ceil_div(rows * (size_t)G, 256)), block(256);
 #define AG_FOLD_ROWS(GG)                                                                                               \
     do {                                                                                                               \
@@ -708,8 +713,11 @@ extern "C" ag_status_t ag_reduce_sum_f32(ag_stream_t stream, const float *x, flo
         bool fits = true;  // launch limits of the streaming kernels
         for (int i = 0; i < pl.n_steps; ++i) {
             const StreamStep &s = pl.step[i];
-            const size_t blocks = s.kind == 0 ? ceil_div(s.outer, 4) : s.kind == 1 ? s.outer * s.splits : ceil_div(s.inner, 256);
-            fits &= blocks < (size_t)kMaxGridX;
+            const bool vec = s.len % 4 == 0 && aligned16(i == 0 ? (const void *)x : ws);
+            const size_t blocks = s.kind == 0   ? ceil_div(s.outer * (size_t)fold_rows_lanes(s.len, vec), 256)
+                                  : s.kind == 1 ? s.outer * s.splits
+                                                : ceil_div(s.inner, s.inner % 4 == 0 && s.len >= 16 ? 128 : 256);
+            fits &= blocks <= (size_t)kMaxGridX;
         }
         if (fits) {
             run_stream(st, pl, x, total, out, static_cast<float *>(ws), scale, do_scale);
