@@ -141,6 +141,24 @@ __global__ __launch_bounds__(kLongT) void rms_norm_long_kernel(NormArgs a)
     }
 }
 
+// Calls launch(arguments, rows) for the rows, `threads` each, as many at a time as a launch holds.
+template <typename F>
+static void norm_in_launches(const NormArgs &a, unsigned rows, unsigned threads, F launch)
+{
+    const unsigned most = (unsigned)(kMaxThreadsX / threads) / 4 * 4;  // (whole blocks of four rows)
+    for (unsigned first = 0; first < rows; first += most) {
+        NormArgs p = a;
+        const size_t cells = (size_t)first * (size_t)a.n;
+        p.x += cells;
+        if (p.residual) p.residual += cells;
+        if (p.h) p.h += cells;
+        if (p.y) p.y += cells;
+        if (p.rstd) p.rstd += first;
+        if (p.q) p.q += (size_t)first * a.nb * kE4m3Block, p.scales += (size_t)first * a.nbp;
+        launch(p, rows - first < most ? rows - first : most);
+    }
+}
+
 // ---- gradient ---------------------------------------------------------------------------------------------------------
 constexpr size_t kStreamBytes = (size_t)256 << 20;  // of one array
 
@@ -332,15 +350,14 @@ extern "C" ag_status_t ag_rms_norm_f32(ag_stream_t stream, const float *x, const
     AG_REQUIRE(aligned16(q), AG_ERR_INVALID_DIMS, "rms_norm: 8-bit output must be 16-byte aligned");
     NormArgs a = {x, residual, weight, h, y, rstd, q, scales, (double)eps, n, (unsigned)(e4m3_pitch(n) / kE4m3Block), (unsigned)e4m3_scale_pitch(n)};
     hipStream_t st = as_stream(stream);
-    const unsigned R = (unsigned)rows;
     // Threads of a row: the padding of the scales (a multiple of 512 elements) has to be covered by the quads.
     const long long cells = (long long)e4m3_scale_pitch(n) * kE4m3Block;
     const bool streams = (size_t)rows * (size_t)n * sizeof(float) >= kStreamBytes;
-#define NORM(T, Q)                                                                                                             \
-    do {                                                                                                                       \
-        if (streams) hipLaunchKernelGGL((rms_norm_kernel<T, Q, true>), dim3(T == 64 ? (R + 3) / 4 : R), dim3(T == 64 ? 256 : T), 0, st, a, R); \
-        else hipLaunchKernelGGL((rms_norm_kernel<T, Q, false>), dim3(T == 64 ? (R + 3) / 4 : R), dim3(T == 64 ? 256 : T), 0, st, a, R);       \
-    } while (0)
+#define NORM(T, Q)                                                                                                                  \
+    norm_in_launches(a, (unsigned)rows, T, [&](const NormArgs &p, unsigned r) {                                                     \
+        if (streams) hipLaunchKernelGGL((rms_norm_kernel<T, Q, true>), dim3(T == 64 ? (r + 3) / 4 : r), dim3(T == 64 ? 256 : T), 0, st, p, r); \
+        else hipLaunchKernelGGL((rms_norm_kernel<T, Q, false>), dim3(T == 64 ? (r + 3) / 4 : r), dim3(T == 64 ? 256 : T), 0, st, p, r);       \
+    })
     if (cells <= 512) NORM(64, 2);
     else if (cells <= 1024) NORM(64, 4);
     else if (cells <= 2048) NORM(256, 2);
@@ -352,7 +369,9 @@ extern "C" ag_status_t ag_rms_norm_f32(ag_stream_t stream, const float *x, const
     else if (cells <= 16384) NORM(1024, 4);
     else if (cells <= 20480) NORM(1024, 5);
     else if (cells <= kMaxRegisterRow) NORM(1024, 8);
-    else hipLaunchKernelGGL(rms_norm_long_kernel, dim3(R), dim3(kLongT), 0, st, a);
+    else
+        norm_in_launches(a, (unsigned)rows, kLongT,
+                         [&](const NormArgs &p, unsigned r) { hipLaunchKernelGGL(rms_norm_long_kernel, dim3(r), dim3(kLongT), 0, st, p); });
 #undef NORM
     return check_launch("rms_norm");
 }

@@ -31,3 +31,24 @@ def test_reduction_of_more_rows_than_a_launch_has(K, n):
     step = 1 << 22
     for i in range(0, rows, step):
         assert torch.equal(got[i:i + step], x[i:i + step].sum(1)), i
+
+
+@pytest.mark.parametrize("rows,n", [(1 << 26, 1), ((1 << 26) + 7, 3)])
+def test_norm_of_more_rows_than_a_launch_has(K, rows, n):
+    say("rms_norm", rows, n)
+    x = torch.randn(rows, n, device="cuda")
+    w, cut = torch.randn(n, device="cuda"), (1 << 26) - 9
+    y, h, rstd = K.rms_norm(x, w, 1e-3, residual=x)
+    for part in (slice(0, 50), slice(cut - 1000, cut + 9), slice(rows - 50, rows)):
+        for got, want in zip((y, h, rstd), K.rms_norm(x[part], w, 1e-3, residual=x[part])):
+            assert same(got[part], want)
+    step = 1 << 22
+    for i in range(0, rows, step):  # every row, against the definition
+        h64 = 2 * x[i:i + step].double()
+        want = h64 * (w.double() / (h64.square().mean(1, keepdim=True) + float(np.float32(1e-3))).sqrt())
+        assert ((y[i:i + step].double() - want).abs() <= 2.0 ** -24 * (1 + 1e-6) * want.abs() + 2.0 ** -149).all()
+    del y, h
+    e, _, _ = K.rms_norm_e4m3(x, w, 1e-3)
+    part = slice(rows - 50, rows)
+    want = K.rms_norm_e4m3(x[part], w, 1e-3)[0]
+    assert same(e.q[part], want.q) and same(e.scales[part], want.scales)
