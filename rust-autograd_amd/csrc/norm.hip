@@ -164,7 +164,7 @@ constexpr size_t kStreamBytes = (size_t)256 << 20;  // of one array
 
 struct NormGradArgs {
     const float *h, *weight, *rstd, *gy, *gh;
-    float *gx, *partial;  // partial: [gridDim.x][n] sums of gw, or null
+    float *gx, *partial;  // partial: [blocks that share the rows][n] sums of gw, or null
     long long n;
 };
 
@@ -251,16 +251,16 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_grad_kernel(NormGr
 // Rows beyond the registers: the weight's sums first (gx may be gy or gh), then gx in two passes over each row.
 __global__ __launch_bounds__(256) void rms_norm_grad_weight_long_kernel(NormGradArgs a, unsigned rows)
 {
-    const long long i = ((long long)blockIdx.y * 256 + threadIdx.x) * 4;
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= a.n) return;
     quad_t acc = {0.f, 0.f, 0.f, 0.f};
-    for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    for (size_t row = blockIdx.y; row < rows; row += gridDim.y) {
         const quad_t h = load_quad(a.h + row * a.n, i, a.n), g = load_quad(a.gy + row * a.n, i, a.n);
         const float r = a.rstd[row];
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[j] = fmaf(g[j], h[j] * r, acc[j]);
     }
-    store_quad(a.partial + (size_t)blockIdx.x * a.n, i, a.n, acc);
+    store_quad(a.partial + (size_t)blockIdx.y * a.n, i, a.n, acc);
 }
 __global__ __launch_bounds__(kLongT) void rms_norm_grad_long_kernel(NormGradArgs a)
 {
@@ -280,13 +280,13 @@ __global__ __launch_bounds__(kLongT) void rms_norm_grad_long_kernel(NormGradArgs
     }
 }
 
-// gw[c] = sum over the G partial rows, in 64 bits: a block has 32 columns, 128 groups of 8 threads take every 128th row
+// gw[c] = sum over the G partial rows, `pitch` elements apart, in 64 bits: a block has 32 columns, 128 groups of 8 threads take every 128th row
 // each (a quad of columns per thread), and the groups are added in order, by eights and then the sixteen sums.  (With 128
 // columns to a block and 32 groups a short row leaves most of the chip idle: the gradient
 // of 20000 x 257 takes 49 us that way and 27 this way, of 2000 x 1023 20 and 15.)
 constexpr int kFoldGroups = 128;
 __global__ __launch_bounds__(kFoldGroups * 8) void rms_norm_grad_fold_kernel(const float *__restrict__ partial, float *__restrict__ gw, long long n,
-                                                                            unsigned G)
+                                                                            long long pitch, unsigned G)
 {
     __shared__ double sums[kFoldGroups][32], eights[kFoldGroups / 8][32];
     const int lane = threadIdx.x & 7, g = threadIdx.x >> 3;
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(kFoldGroups * 8) void rms_norm_grad_fold_kernel(con
     if (i < n)
 #pragma unroll 4
         for (unsigned b = g; b < G; b += kFoldGroups) {
-            const quad_t v = load_quad(partial + (size_t)b * n, i, n);
+            const quad_t v = load_quad(partial + (size_t)b * pitch, i, n);
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[j] += (double)v[j];
         }
@@ -398,6 +398,7 @@ extern "C" ag_status_t ag_rms_norm_grad_f32(ag_stream_t stream, const float *h, 
     AG_REQUIRE(!gw || (ws && ws_bytes >= ag_rms_norm_grad_f32_workspace(rows, n)), AG_ERR_INVALID_DIMS,
                "rms_norm_grad: workspace of %zu bytes, %zu needed", ws_bytes, ag_rms_norm_grad_f32_workspace(rows, n));
     AG_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 3u) == 0, AG_ERR_INVALID_DIMS, "rms_norm_grad: misaligned workspace");
+    AG_REQUIRE(n <= 16384 || rows <= kMaxThreadsX / kLongT, AG_ERR_INVALID_DIMS, "rms_norm_grad: %d rows of %d elements", rows, n);
     const unsigned R = (unsigned)rows, G = norm_grad_blocks(rows, n);
     NormGradArgs a = {h, weight, rstd, gy, gh, gx, gw ? static_cast<float *>(ws) : nullptr, n};
     const bool streams = (size_t)rows * (size_t)n * sizeof(float) >= kStreamBytes;
@@ -415,12 +416,17 @@ extern "C" ag_status_t ag_rms_norm_grad_f32(ag_stream_t stream, const float *h, 
     else if (n <= 8192) GRAD(512, 4);
     else if (n <= 16384) GRAD(1024, 4);
     else {
-        if (gw) hipLaunchKernelGGL(rms_norm_grad_weight_long_kernel, dim3(G, (unsigned)((n + 1023) / 1024)), dim3(256), 0, st, a, R);
+        if (gw) hipLaunchKernelGGL(rms_norm_grad_weight_long_kernel, dim3((unsigned)(((long long)n + 1023) / 1024), G), dim3(256), 0, st, a, R);
         if (gx) hipLaunchKernelGGL(rms_norm_grad_long_kernel, dim3(R), dim3(kLongT), 0, st, a);
     }
 #undef GRAD
-    if (gw)
-        hipLaunchKernelGGL(rms_norm_grad_fold_kernel, dim3((unsigned)((n + 31) / 32)), dim3(kFoldGroups * 8), 0, st,
-                           static_cast<const float *>(ws), gw, n, G);
+    if (gw) {
+        constexpr long long most = kMaxThreadsX / (kFoldGroups * 8) * 32;  // columns of a launch
+        for (long long c = 0; c < n; c += most) {
+            const long long count = n - c < most ? n - c : most;
+            hipLaunchKernelGGL(rms_norm_grad_fold_kernel, dim3((unsigned)((count + 31) / 32)), dim3(kFoldGroups * 8), 0, st,
+                               static_cast<const float *>(ws) + c, gw + c, count, (long long)n, G);
+        }
+    }
     return check_launch("rms_norm_grad");
 }

@@ -52,3 +52,21 @@ def test_norm_of_more_rows_than_a_launch_has(K, rows, n):
     part = slice(rows - 50, rows)
     want = K.rms_norm_e4m3(x[part], w, 1e-3)[0]
     assert same(e.q[part], want.q) and same(e.scales[part], want.scales)
+
+
+@pytest.mark.parametrize("rows,n", [(1, (1 << 26) + 5), (2, (1 << 27) + 5)])
+def test_norm_gradient_of_more_columns_than_a_launch_has(K, rows, n):
+    say("rms_norm_grad", rows, n)
+    h, gy = torch.randn(rows, n, device="cuda"), torch.randn(rows, n, device="cuda")
+    w, rstd = torch.randn(n, device="cuda"), torch.full((rows,), 0.75, device="cuda")
+    gx, gw = K.rms_norm_grad(h, w, rstd, gy)
+    c = [(gy[i].double() * w.double() * h[i].double()).sum() / n * 0.75 ** 3 for i in range(rows)]
+    step = 1 << 24
+    for i in range(0, n, step):
+        s = slice(i, i + step)
+        h64, g64, w64 = h[:, s].double(), gy[:, s].double(), w[s].double()
+        first, second = 0.75 * w64 * g64, torch.stack([h64[r] * c[r] for r in range(rows)])
+        # one rounding of gx (6 u cover the order of c's sum); of gw two roundings a term, `rows` of the sum, one of the result
+        assert ((gx[:, s].double() - (first - second)).abs() <= 6 * 2.0 ** -24 * (first.abs() + second.abs()) + 2.0 ** -149).all()
+        terms = g64 * h64 * 0.75
+        assert ((gw[s].double() - terms.sum(0)).abs() <= (rows + 4) * 2.0 ** -24 * terms.abs().sum(0) + 2.0 ** -149).all()

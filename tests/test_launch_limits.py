@@ -34,3 +34,8 @@ def test_adam_of_many_elements(L):
     refused(L, L.ag_adam_update_f32(N, P, P, P, P, P, 1 << 36, 1e-3, 1e-8, 0.9, 0.999), "too many elements")
     at = [(C.c_void_p * 1)(4096 * (i + 1)) for i in range(5)]
     refused(L, L.ag_adam_update_multi_f32(N, 1, *at, (C.c_size_t * 1)(1 << 36), 1e-3, 1e-8, 0.9, 0.999), "too many elements")
+
+
+def test_norm_gradient_of_many_long_rows(L):
+    other = C.c_void_p(8192)
+    refused(L, L.ag_rms_norm_grad_f32(N, P, P, P, P, N, other, N, 1 << 22, 16385, N, 0), "4194304 rows of 16385")
