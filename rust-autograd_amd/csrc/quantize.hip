@@ -46,13 +46,13 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const float *__restr
 __global__ __launch_bounds__(256) void quantize_tile_kernel(const float *__restrict__ x, long long ldx, int rows, int cols,
                                                             unsigned char *__restrict__ q, unsigned char *__restrict__ scales,
                                                             unsigned char *__restrict__ qt, unsigned char *__restrict__ scales_t, unsigned nb,
-                                                            unsigned nbp, unsigned mb, unsigned mbp)
+                                                            unsigned nbp, unsigned mb, unsigned mbp, unsigned first)
 {
     constexpr int kPitch = kE4m3Block + 16;
     __shared__ __attribute__((aligned(16))) unsigned colmax[8][kE4m3Block];
     __shared__ __attribute__((aligned(16))) unsigned char turned[kE4m3Block * kPitch];
     const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
-    const unsigned tb = blockIdx.x % nb, tm = blockIdx.x / nb;  // block column, block row
+    const unsigned tile = first + blockIdx.x, tb = tile % nb, tm = tile / nb;  // block column, block row
     const long long m0 = (long long)tm * kE4m3Block + g * 16;
     const long long c0 = (long long)tb * kE4m3Block;
     quad_t v[16];
@@ -140,17 +140,20 @@ ag_status_t quantize_e4m3(const char *who, hipStream_t st, const float *x, long 
     if (rows == 0 || cols == 0) return AG_OK;
     const unsigned nb = (unsigned)(e4m3_pitch(cols) / kE4m3Block), nbp = (unsigned)e4m3_scale_pitch(cols);
     if (!qt) {
-        const unsigned long long items = (unsigned long long)rows * nbp;
-        AG_REQUIRE(items < (1ull << 32) - 64, AG_ERR_INVALID_DIMS, "%s: too many blocks (%llu)", who, items);
-        const unsigned per = 8u * kRowsPerThread;
-        hipLaunchKernelGGL(quantize_rows_kernel, dim3((unsigned)((items + per - 1) / per)), dim3(256), 0, st, x, ldx, cols, q, scales, nb, nbp,
-                           (unsigned)items);
+        // 8 threads to an item; rows as many at a time as a launch holds (a row has at most 2^24 items)
+        const unsigned per = 8u * kRowsPerThread, most = (unsigned)(kMaxThreadsX / 8 - per) / nbp;
+        for (unsigned r = 0; r < (unsigned)rows; r += most) {
+            const unsigned items = ((unsigned)rows - r < most ? (unsigned)rows - r : most) * nbp;
+            hipLaunchKernelGGL(quantize_rows_kernel, dim3((items + per - 1) / per), dim3(256), 0, st, x + r * ldx, ldx, cols,
+                               q + (size_t)r * nb * kE4m3Block, scales + (size_t)r * nbp, nb, nbp, items);
+        }
     } else {
         const unsigned mb = (unsigned)(e4m3_pitch(rows) / kE4m3Block), mbp = (unsigned)e4m3_scale_pitch(rows);
-        const unsigned long long tiles = (unsigned long long)nb * mb;
-        AG_REQUIRE(tiles <= (unsigned long long)kMaxGridX, AG_ERR_INVALID_DIMS, "%s: too many blocks (%llu)", who, tiles);
-        hipLaunchKernelGGL(quantize_tile_kernel, dim3((unsigned)tiles), dim3(256), 0, st, x, ldx, rows, cols, q, scales, qt, scales_t, nb, nbp, mb,
-                           mbp);
+        const unsigned long long tiles = (unsigned long long)nb * mb, most = kMaxGridX;
+        AG_REQUIRE(tiles < (1ull << 32) - most, AG_ERR_INVALID_DIMS, "%s: too many blocks (%llu)", who, tiles);
+        for (unsigned long long t = 0; t < tiles; t += most)
+            hipLaunchKernelGGL(quantize_tile_kernel, dim3((unsigned)(tiles - t < most ? tiles - t : most)), dim3(256), 0, st, x, ldx, rows, cols, q,
+                               scales, qt, scales_t, nb, nbp, mb, mbp, (unsigned)t);
     }
     return check_launch(who);
 }

@@ -70,3 +70,29 @@ def test_norm_gradient_of_more_columns_than_a_launch_has(K, rows, n):
         assert ((gx[:, s].double() - (first - second)).abs() <= 6 * 2.0 ** -24 * (first.abs() + second.abs()) + 2.0 ** -149).all()
         terms = g64 * h64 * 0.75
         assert ((gw[s].double() - terms.sum(0)).abs() <= (rows + 4) * 2.0 ** -24 * terms.abs().sum(0) + 2.0 ** -149).all()
+
+
+def test_rounding_of_more_rows_than_a_launch_has(K):
+    rows = (1 << 27) + 3
+    say("quantize", rows, 1)
+    x = torch.randn(rows, 1, device="cuda")
+    e = K.quantize_e4m3(x)
+    step = 1 << 22
+    for i in range(0, rows, step):  # (a row of one element: its block's largest is itself)
+        part = K.quantize_e4m3(x[i:i + step])
+        assert same(e.q[i:i + step], part.q) and same(e.scales[i:i + step], part.scales), i
+
+
+def test_rounding_of_a_column_of_more_blocks_than_a_launch_has(K):
+    rows = (1 << 31) - 1
+    say("quantize, transposed", rows, 1)
+    x = torch.empty(rows, 1, device="cuda").normal_()
+    t = K.quantize_e4m3(x, transpose=True)
+    for i in (0, (1 << 31) - (1 << 20)):  # whole blocks, the last one ragged
+        part = K.quantize_e4m3(x[i:i + (1 << 20)].t().contiguous())
+        assert same(t.q[:, i:i + (1 << 20)], part.q)
+        assert same(t.scales[:, i // 128:i // 128 + part.scales.shape[1]], part.scales)
+    # every block: rounded along the rows of the array cut into rows of whole blocks
+    whole = rows // 512 * 512
+    cut = K.quantize_e4m3(x[:whole].view(-1, 512))
+    assert same(t.q[0, :whole].view(-1, 512), cut.q) and same(t.scales[0, :whole // 128].view(-1, 4), cut.scales)
