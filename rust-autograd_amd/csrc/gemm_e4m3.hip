@@ -457,20 +457,37 @@ static ag_status_t check_product(const char *who, int M, int N, int K, int ldc, 
     AG_REQUIRE(c && (K == 0 || (b && bs)), AG_ERR_INVALID_DIMS, "%s: null pointer", who);
     AG_REQUIRE(aligned16(b), AG_ERR_INVALID_DIMS, "%s: 8-bit operands must be 16-byte aligned", who);
     AG_REQUIRE((reinterpret_cast<uintptr_t>(bs) & 3u) == 0, AG_ERR_INVALID_DIMS, "%s: scales must be 4-byte aligned", who);
+    const Plan f = plan_product(M, N, K);
+    if (f.tile == 0) return AG_OK;
+    // (the places of a tile's rows and columns are 32-bit ints, behind the last row too)
+    AG_REQUIRE(M <= 0x7fffffff - 512 && N <= 0x7fffffff - 512, AG_ERR_INVALID_DIMS, "%s: operands of %d and %d rows", who, M, N);
+    const long long tiles = (long long)((M + f.tile - 1) / f.tile) * ((N + f.tile - 1) / f.tile) * f.splits;
+    AG_REQUIRE(tiles <= kMaxThreadsX / (f.tile == 256 ? 512 : 256), AG_ERR_INVALID_DIMS, "%s: too many tiles (%lld)", who, tiles);
     return AG_OK;
 }
 
+template <int MT, int NW, int XR>
+static void launch_skinny_waves(hipStream_t st, GemmE4m3 p, const float *x, long long ldx, int K)
+{
+    // columns as many at a time as a launch holds
+    constexpr int most = (int)(kMaxThreadsX / (NW * 64) * 16 < 0x7ffffff0LL ? kMaxThreadsX / (NW * 64) * 16 : 0x7ffffff0LL);
+    const int N = p.N;
+    for (int done = 0;; done += most) {
+        p.N = N - done < most ? N - done : most;
+        hipLaunchKernelGGL((gemm_e4m3_skinny_kernel<MT, NW, XR>), dim3((unsigned)((p.N + 15) / 16)), dim3(NW * 64), 0, st, p, x, ldx, K);
+        if (N - done <= most) return;
+        p.b += most * p.pitch;
+        p.b_scales += (long long)most * p.scale_pitch;
+        p.c += most;
+    }
+}
 template <int MT, int XR>
 static void launch_skinny(hipStream_t st, const GemmE4m3 &p, const float *x, long long ldx, int K)
 {
-    const dim3 grid((unsigned)((p.N + 15) / 16));
     const int words = (p.blocks + 3) / 4;  // a wave each, up to eight
-    if (words <= 2)
-        hipLaunchKernelGGL((gemm_e4m3_skinny_kernel<MT, 2, XR>), grid, dim3(128), 0, st, p, x, ldx, K);
-    else if (words <= 4)
-        hipLaunchKernelGGL((gemm_e4m3_skinny_kernel<MT, 4, XR>), grid, dim3(256), 0, st, p, x, ldx, K);
-    else
-        hipLaunchKernelGGL((gemm_e4m3_skinny_kernel<MT, 8, XR>), grid, dim3(512), 0, st, p, x, ldx, K);
+    if (words <= 2) launch_skinny_waves<MT, 2, XR>(st, p, x, ldx, K);
+    else if (words <= 4) launch_skinny_waves<MT, 4, XR>(st, p, x, ldx, K);
+    else launch_skinny_waves<MT, 8, XR>(st, p, x, ldx, K);
 }
 
 static ag_status_t product(const char *who, hipStream_t st, GemmE4m3 p, int K, void *ws)
@@ -485,19 +502,18 @@ static ag_status_t product(const char *who, hipStream_t st, GemmE4m3 p, int K, v
     p.tiles_n = (p.N + f.tile - 1) / f.tile;
     p.splits = f.splits;
     p.per_split = (p.blocks + f.splits - 1) / f.splits;
-    const unsigned long long grid = (unsigned long long)p.tiles_m * p.tiles_n * f.splits;
-    AG_REQUIRE(grid <= (unsigned long long)kMaxGridX, AG_ERR_INVALID_DIMS, "%s: too many tiles (%llu)", who, grid);
+    const unsigned grid = (unsigned)p.tiles_m * p.tiles_n * f.splits;
     float *c = p.c;
     const long long ldc = p.ldc;
     if (f.splits > 1) p.c = static_cast<float *>(ws), p.ldc = p.N;
     if (f.tile == 256)
-        hipLaunchKernelGGL((gemm_e4m3_tile_kernel<256, 256, 128, 64, 2>), dim3((unsigned)grid), dim3(512), 0, st, p);
+        hipLaunchKernelGGL((gemm_e4m3_tile_kernel<256, 256, 128, 64, 2>), dim3(grid), dim3(512), 0, st, p);
     else if (f.tile == 128 && f.deep)
-        hipLaunchKernelGGL((gemm_e4m3_tile_kernel<128, 128, 64, 64, 4>), dim3((unsigned)grid), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((gemm_e4m3_tile_kernel<128, 128, 64, 64, 4>), dim3(grid), dim3(256), 0, st, p);
     else if (f.tile == 128)
-        hipLaunchKernelGGL((gemm_e4m3_tile_kernel<128, 128, 64, 64, 2>), dim3((unsigned)grid), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((gemm_e4m3_tile_kernel<128, 128, 64, 64, 2>), dim3(grid), dim3(256), 0, st, p);
     else
-        hipLaunchKernelGGL((gemm_e4m3_tile_kernel<64, 64, 32, 32, 4>), dim3((unsigned)grid), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((gemm_e4m3_tile_kernel<64, 64, 32, 32, 4>), dim3(grid), dim3(256), 0, st, p);
     if (f.splits > 1) {
         const long long cells = (long long)p.M * p.N;
         hipLaunchKernelGGL(gemm_e4m3_fold_kernel, dim3((unsigned)((cells + 1023) / 1024)), dim3(256), 0, st, static_cast<const float *>(ws), c, ldc, p.M,

@@ -96,3 +96,24 @@ def test_rounding_of_a_column_of_more_blocks_than_a_launch_has(K):
     whole = rows // 512 * 512
     cut = K.quantize_e4m3(x[:whole].view(-1, 512))
     assert same(t.q[0, :whole].view(-1, 512), cut.q) and same(t.scales[0, :whole // 128].view(-1, 4), cut.scales)
+
+
+def test_product_of_more_columns_than_a_launch_has(K):
+    n, k, m = (1 << 29) + 21, 8, 3
+    say("product", m, n, k)
+    rng = np.random.default_rng(3)
+    a = dev(rng.integers(-3, 4, (m, k)))
+    b = torch.empty(n, 128, dtype=torch.uint8, device="cuda").zero_()
+    step = 1 << 20
+    values = K.quantize_e4m3(dev(rng.integers(-3, 4, (step, k))))
+    for i in range(0, n, step):
+        b[i:i + step].copy_(values.q.view(torch.uint8)[: n - i])
+    scales = torch.full((n, 4), 127, dtype=torch.uint8, device="cuda")
+    power = values.scales.view(torch.uint8)[:, 0]
+    for i in range(0, n, step):
+        scales[i:i + step, 0].copy_(power[: n - i])
+    e = K.E4m3(b.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu), k)
+    want = (a.double() @ values.values().double().t()).float()  # integers: exact
+    for got in (K.quantize_matmul_e4m3(a, e), K.matmul_e4m3(K.quantize_e4m3(a), e)):
+        for i in range(0, n, step):
+            assert torch.equal(got[:, i:i + step], want[:, : n - i]), i

@@ -39,3 +39,13 @@ def test_adam_of_many_elements(L):
 def test_norm_gradient_of_many_long_rows(L):
     other = C.c_void_p(8192)
     refused(L, L.ag_rms_norm_grad_f32(N, P, P, P, P, N, other, N, 1 << 22, 16385, N, 0), "4194304 rows of 16385")
+
+
+def test_product_of_many_tiles_and_of_rows_at_the_end_of_an_int(L):
+    # K = 0: no operand is read
+    most = 2 ** 31 - 1
+    f = L.ag_matmul_e4m3_f32
+    refused(L, f(N, most - 512, 300, 0, N, N, N, N, P, 300, N, 0), "too many tiles")
+    refused(L, f(N, 20, most, 4096, P, P, P, P, P, most, N, 0), "operands of 20 and 2147483647 rows")
+    refused(L, f(N, most, 20, 4096, P, P, P, P, P, 20, N, 0), "operands of 2147483647 and 20 rows")
+    refused(L, L.ag_quantize_matmul_e4m3_f32(N, 20, most, 4096, P, 4096, P, P, P, most, P, 1 << 40), "operands of 20 and")
