@@ -553,10 +553,17 @@ def _here(t, name, dtype=torch.float32):
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _ints(name, rows, n):
+    """Refuses extents that the C ABI's ints do not hold (ctypes would pass the low 32 bits)."""
+    if rows > 0x7FFFFFFF or n > 0x7FFFFFFF:
+        raise capi.InvalidDims(f"{name}: extents {rows} and {n} (at most 2147483647)")
+
+
 def _matrix(x, name):
     x = _here(x, name)
     if x.dim() != 2:
         raise capi.IncompatibleShape(f"{name}: input must be 2D (got {list(x.shape)})")
+    _ints(name, *x.shape)
     return x
 
 
@@ -572,6 +579,7 @@ def _e4m3(e, name):
     q, scales = _here(e.q, name, torch.float8_e4m3fn), _here(e.scales, name, torch.float8_e8m0fnu)
     if q.dim() != 2 or q.shape[1] != -(-e.n // 128) * 128 or scales.shape != (q.shape[0], -(-e.n // 512) * 4):
         raise capi.IncompatibleShape(f"{name}: values {list(q.shape)} and scales {list(scales.shape)} are not those of rows of {e.n} elements")
+    _ints(name, q.shape[0], e.n)
     return q, scales, q.shape[0], e.n
 
 
@@ -634,14 +642,15 @@ def _rms_norm(x, weight, eps, residual, e4m3):
     x, weight = _here(x, "rms_norm"), _here(weight, "rms_norm")
     if x.dim() < 1 or weight.dim() != 1 or weight.shape[0] != x.shape[-1]:
         raise capi.IncompatibleShape(f"rms_norm: weight {list(weight.shape)} for rows of {list(x.shape)}")
+    n = x.shape[-1]
+    rows = x.numel() // n if n else 0
+    _ints("rms_norm", rows, n)
     h, res = x, None
     if residual is not None:
         res = _here(residual, "rms_norm")
         if res.shape != x.shape:
             raise capi.IncompatibleShape(f"rms_norm: residual {list(res.shape)} and input {list(x.shape)}")
         h = torch.empty_like(x)
-    n = x.shape[-1]
-    rows = x.numel() // n if n else 0
     rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
     if e4m3:
         y = _e4m3_empty(rows, n, x.device)
@@ -673,6 +682,7 @@ def rms_norm_grad(h, weight, rstd, gy, gh=None):
     if weight.shape != (n,) or rstd.shape != (rows,) or gy.shape != h.shape:
         raise capi.IncompatibleShape(f"rms_norm_grad: h {list(h.shape)}, weight {list(weight.shape)}, rstd {list(rstd.shape)}, "
                                      f"gy {list(gy.shape)}")
+    _ints("rms_norm_grad", rows, n)
     if gh is not None:
         gh = _here(gh, "rms_norm_grad")
         if gh.shape != h.shape:

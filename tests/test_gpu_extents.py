@@ -117,3 +117,20 @@ def test_product_of_more_columns_than_a_launch_has(K):
     for got in (K.quantize_matmul_e4m3(a, e), K.matmul_e4m3(K.quantize_e4m3(a), e)):
         for i in range(0, n, step):
             assert torch.equal(got[:, i:i + step], want[:, : n - i]), i
+
+
+def test_extents_beyond_32_bits_are_refused(K):
+    """2^32 + 8 rows would reach the library as 8."""
+    from rust_autograd_amd import capi
+
+    rows = (1 << 32) + 8
+    x, w = torch.zeros(rows, 1, device="cuda"), torch.ones(1, device="cuda")
+    byte, scales = torch.zeros(4, 128, dtype=torch.uint8, device="cuda"), torch.full((4, 4), 127, dtype=torch.uint8, device="cuda")
+    e = K.E4m3(byte.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu), 1)
+    for call in (lambda: K.rms_norm(x, w), lambda: K.rms_norm_e4m3(x, w), lambda: K.rms_norm_grad(x, w, x[:, 0], x), lambda: K.quantize_e4m3(x),
+                 lambda: K.quantize_e4m3(x, transpose=True), lambda: K.quantize_e4m3(x.view(1, rows)), lambda: K.quantize_e4m3_both(x),
+                 lambda: K.quantize_matmul_e4m3(x, e)):
+        before = torch.cuda.memory_allocated()
+        with pytest.raises(capi.InvalidDims, match="2147483647"):
+            call()
+        assert torch.cuda.memory_allocated() == before
