@@ -743,16 +743,30 @@ def clip_by_global_norm(xs, max_norm, outs=None):
     return outs, clip
 
 
+def _adam_shares_nothing(params, grads, ms, vs, ts, ns):
+    """What the library refuses within one launch, for all of several: two parameters with an array or a step counter in
+    common, and a gradient that is an array another parameter updates."""
+    filled = [i for i, n in enumerate(ns) if n]
+    shared = len(set(ts)) < len(ns) or any(len({a[i] for i in filled}) < len(filled) for a in (params, ms, vs))
+    owner = {a[i]: i for a in (params, ms, vs) for i in filled}
+    if shared or any(owner.get(grads[i], i) != i for i in filled):
+        raise capi.InvalidDims("adam: parameters share an array; update them in separate calls")
+
+
 def adam_update_clipped(params, grads, ms, vs, ts, max_norm, alpha=1e-3, eps=1e-8, b1=0.9, b2=0.999):
     """One optimizer step on gradients clipped to max_norm over all of them, in place on params, ms, vs, ts (any number of
     parameters); the gradients themselves are left as they are.  Returns [norm, coefficient] on the device."""
     ns = _sizes(grads, "adam")
     if any(_sizes(xs, "adam") != ns for xs in (params, ms, vs)) or len(ts) != len(ns) or any(t < 1 for t in _sizes(ts, "adam")):
         raise capi.IncompatibleShape("adam: parameter, gradient and moment sizes differ")
-    clip, table = _global_norm(grads, ns, max_norm)
-    tables = [_pointers(xs) for xs in (params, grads, ms, vs, ts)] + [table]
     L = capi.lib()
-    n, most, word, st, pc = len(ns), L.ag_adam_update_multi_max(), C.sizeof(C.c_void_p), _stream(), clip.data_ptr()
+    n, most, word, st = len(ns), L.ag_adam_update_multi_max(), C.sizeof(C.c_void_p), _stream()
+    tables = [_pointers(xs) for xs in (params, grads, ms, vs, ts)]
+    if n > most:
+        _adam_shares_nothing(*tables, ns)
+    clip, table = _global_norm(grads, ns, max_norm)
+    tables.append(table)
+    pc = clip.data_ptr()
     for i in range(0, n, most):
         check(L.ag_adam_update_multi_clipped_f32(st, min(most, n - i), *[C.byref(t, i * word) for t in tables], alpha, eps, b1, b2, pc))
     return clip

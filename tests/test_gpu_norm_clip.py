@@ -346,3 +346,27 @@ def test_a_captured_step_repeats_the_eager_one(K, rng):
             assert torch.equal(p, q), f"replay {i}"
         for name in start:
             assert all(torch.equal(p, q) for p, q in zip(a[name], b[name])), f"replay {i}: {name}"
+
+
+def test_clipped_adam_refuses_arrays_shared_between_its_launches(K):
+    """More parameters than one launch takes, two of them with one step counter, parameter or moment, or a gradient that is
+    another's parameter: refused before anything is written, as within one launch."""
+    from rust_autograd_amd import capi
+    count = capi.lib().ag_adam_update_multi_max() + 6
+
+    def state():
+        r = np.random.default_rng(5)
+        return [[dev(r.random(40)) for _ in range(count)] for _ in range(4)] + [[torch.ones(1, device="cuda") for _ in range(count)]]
+
+    for table, of in ((0, 0), (2, 2), (3, 3), (4, 4), (1, 0), (1, 2)):
+        for first, last in ((1, count - 2), (count - 1, 0)):
+            s = state()
+            s[table][last] = s[of][first]
+            keep = [[t.clone() for t in ts] for ts in s]
+            with pytest.raises(capi.InvalidDims, match="separate calls"):
+                K.adam_update_clipped(*s, 0.5)
+            assert all(torch.equal(p, q) for a, b in zip(s, keep) for p, q in zip(a, b)), (table, of, first, last)
+    s = state()
+    s[1][count - 1] = s[1][0]  # (a gradient of two parameters is only read)
+    K.adam_update_clipped(*s, 0.5)
+    assert all(t.item() == 2.0 for t in s[4])
