@@ -1550,8 +1550,9 @@ struct RmsNorm : Op {
         if (ctx.input_shape(2).size() != 1 || ctx.input_shape(2)[0] != ctx.input_shape(0).back()) return false;
         const NdArray a = ctx.input(0), b = ctx.input(1), w = ctx.input(2);
         const NdArray h = NdArray::empty(a.shape());
-        *status = run(ctx, a, b, w, h);
-        if (status->ok()) producer_outputs->push_back(h);
+        if (!run(ctx, a, b, w, h).ok()) return false;  // (the norm's error is its own: the sum has a value)
+        *status = OpError::none();
+        producer_outputs->push_back(h);
         return true;
     }
     void grad(GradientContext &ctx) const override

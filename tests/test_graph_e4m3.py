@@ -356,3 +356,16 @@ def test_a_norm_keeps_the_pass_of_the_sum_where_its_weight_is_trained_behind_it(
     assert c.fused_pairs == 1 and np.array_equal(hv, a + b) and not np.array_equal(env.array(w), old)
     want = plain64.rms_norm(hv, old, float(np.float32(1e-6)))[0]
     assert (np.abs(yv - want) <= U * (1 + 1e-6) * np.abs(want)).all()
+
+
+@pytest.mark.gpu
+def test_a_sum_is_evaluated_where_the_norm_behind_it_is_refused(G):
+    """Rows of one element, more of them than the norm takes: its error is its own, the sum in front of it has a value."""
+    env, c = context(G)
+    shape = [1 << 16, (1 << 15) + 1]  # 2^31 + 2^16 elements, a product of two vectors
+    a = c.matmul(c.variable(env.set("a", np.ones((shape[0], 1)))), c.variable(env.set("b", np.full((1, shape[1]), 1.5))))
+    x = c.reshape(a, [shape[0] * shape[1], 1])
+    h = x + x
+    total, y = c.eval([c.reduce_mean(c.reshape(h, shape), [0, 1], False), c.rms_norm(h, c.variable(env.set("w", np.ones(1))))])
+    assert isinstance(y, G.OpError) and y.kind == "InvalidDims" and "rms_norm" in y.message
+    assert abs(float(np.reshape(total, -1)[0]) - 3.0) < 1e-4
