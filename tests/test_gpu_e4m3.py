@@ -283,3 +283,44 @@ def test_offsets_beyond_32_bits(K, rng):
     norm = np.sqrt((host(tail) ** 2).sum() * 5)  # h is twice x
     assert abs(host(clip)[0] - norm) <= 2.0 ** -24 * (1 + 1e-6) * norm
     assert torch.equal(x[-last:], tail * clip[1]) and torch.equal(h[-last:], h1 * clip[1])
+
+
+# ---- every form of the product, by the number of CUs ------------------------------------------------------------------
+def form(m, n, k, cus):
+    """The form that the extents choose: (tile, steps in flight, whether the contraction is sliced), tile 0 for few rows."""
+    steps = -(-k // 128)
+
+    def tiles(t):
+        return -(-m // t) * -(-n // t)
+
+    if m <= 16 or (m <= 32 and n <= 16 * cus and steps <= 32):
+        return 0, 16 if m <= 16 else 32, False
+    if tiles(64) <= 2 * cus:
+        return 64, 4, min(cus // tiles(64), steps // 8) > 1
+    if tiles(128) <= cus:
+        return 128, 4, False
+    return (128, 2, False) if -(-tiles(128) // (2 * cus)) * 62 < -(-tiles(256) // cus) * 100 else (256, 2, False)
+
+
+def cus():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+def a_tile_of_128_per_cu():
+    """Ragged extents of as many tiles of 128 as there are CUs."""
+    return 8 * 128 - 4, cus() // 8 * 128 - 6
+
+
+@pytest.mark.parametrize("k", [1, 100, 128, 256, 300, 512, 640, 768, 1025, 1300])
+def test_tiles_of_128_four_steps_deep(K, rng, k):
+    """One to eleven steps through a ring of four."""
+    m, n = a_tile_of_128_per_cu()
+    assert form(m, n, k, cus()) == (128, 4, False)
+    test_product_of_integers_is_exact(K, rng, m, n, k)
+    if k > 1:
+        test_product_within_the_roundings_of_its_sums(K, rng, m, n, k)
+
+
+def test_the_extents_of_these_tests_reach_every_form():
+    reached = {form(m, n, k, cus()) for m, n, k in PRODUCTS} | {form(*a_tile_of_128_per_cu(), 768, cus())}
+    assert reached == {(0, 16, False), (0, 32, False), (64, 4, False), (64, 4, True), (128, 4, False), (128, 2, False), (256, 2, False)}

@@ -370,3 +370,43 @@ def test_clipped_adam_refuses_arrays_shared_between_its_launches(K):
     s[1][count - 1] = s[1][0]  # (a gradient of two parameters is only read)
     K.adam_update_clipped(*s, 0.5)
     assert all(t.item() == 2.0 for t in s[4])
+
+
+# ---- forms of the norm that the widths above do not reach ---------------------------------------------------------------
+@pytest.mark.parametrize("n", [2560, 2561, 5120, 5121, 5125, 5632, 5633, 6143, 6144, 6145, 20480, 20481])
+@pytest.mark.parametrize("rows,with_residual", [(1, True), (5, False), (6, True)])
+def test_norm_at_the_borders_of_its_forms(K, rng, rows, with_residual, n):
+    test_norm_is_the_formula_rounded_once(K, rng, rows, with_residual, n)
+
+
+@pytest.mark.parametrize("n", [6143, 6144, 6145])
+def test_norm_gradient_at_the_borders_of_its_forms(K, rng, n):
+    test_norm_gradient_is_the_formula(K, rng, 7, True, n)
+
+
+@pytest.mark.parametrize("n", [130, 511, 1023, 2046, 2555, 4091, 5115, 6130, 8190, 16380, 20470, 32761, 33001])
+def test_arrays_beyond_the_caches_have_the_bits_of_their_parts(K, rng, n):
+    """Arrays of 256 MiB and more are read past the caches."""
+    rows = (1 << 26) // n + 5
+    say("large", rows, n)
+    x, res, gy = (torch.randn(rows, n, device="cuda") for _ in range(3))
+    w = torch.randn(n, device="cuda")
+    y, h, rstd = K.rms_norm(x, w, 1e-6, residual=res)
+    e, _, _ = K.rms_norm_e4m3(x, w, 1e-6, residual=res)
+    gx, gw = K.rms_norm_grad(h, w, rstd, gy, gh=res)
+    sums, sizes = torch.zeros(n, dtype=torch.float64, device="cuda"), torch.zeros(n, dtype=torch.float64, device="cuda")
+    step = -(-rows // 4)
+    for i in range(0, rows, step):
+        s = slice(i, i + step)
+        y1, h1, rstd1 = K.rms_norm(x[s], w, 1e-6, residual=res[s])
+        e1, _, _ = K.rms_norm_e4m3(x[s], w, 1e-6, residual=res[s])
+        gx1, _ = K.rms_norm_grad(h1, w, rstd1, gy[s], gh=res[s])
+        for got, want in ((y[s], y1), (h[s], h1), (rstd[s], rstd1), (gx[s], gx1), (e.q[s].view(torch.uint8), e1.q.view(torch.uint8)),
+                          (e.scales[s].view(torch.uint8), e1.scales.view(torch.uint8))):
+            assert torch.equal(got, want)
+        terms = gy[s].double() * h1.double() * rstd1.double()[:, None]
+        sums += terms.sum(0)
+        sizes += terms.abs().sum(0)
+    # (a block adds its rows in f32 in turn: at most all of them)
+    assert ((gw.double() - sums).abs() <= (rows + 4) * U * sizes + TINY).all()
+    torch.cuda.empty_cache()
