@@ -387,14 +387,18 @@ size_t ag_e4m3_scale_pitch(int n);
 /* Rounds x [rows, cols] (row stride ldx) to such operands: along its rows into q, scales, along its columns into qt
  * [cols, ag_e4m3_pitch(rows)] and scales_t (the transposed array); either pair may be NULL, one pass over x serves both.
  * The scale of a block is the smallest power of two, at least 2^-117, with the block's largest finite magnitude at most
- * 448 times it (1 for a block of zeros); elements are rounded to nearest, ties to even.  An element that is not finite
+ * 448 times it (1 for a block of zeros); elements are rounded to nearest, ties to even.  (Bytes are thus 10 to 247.  A
+ * magnitude of 1.9375 * 2^127 and more is rounded to 2^128, which an f32 does not hold.)  An element that is not finite
  * becomes NaN and takes no part in the scale.  q and qt are 16-byte aligned. */
 ag_status_t ag_quantize_e4m3_f32(ag_stream_t stream, const float *x, int ldx, int rows, int cols, uint8_t *q,
                                  uint8_t *scales, uint8_t *qt, uint8_t *scales_t);
 
 /* C[M x N] = A . B^T of the 8-bit operands A (M rows) and B (N rows), K elements along the contraction, f32 accumulation
- * and output, row stride ldc.  Each product of two blocks is exact; sums are f32 in an order that depends on the extents
- * only.  A NaN reaches the elements that it takes part in.  With a [M,K], b [K,N] and y = a . b, and each operand rounded
+ * and output, row stride ldc.  An element enters as q * scale in bf16, exactly with the bytes 10 to 247 that rounding
+ * writes, 2^128 as an infinity; operands from elsewhere may hold other bytes, and what bf16 does not hold is then lost:
+ * multiples of less than 2^-133 are rounded to such, 2^128 and more count as infinities, byte 255 as NaN.  Each product of
+ * two elements is exact but for f32's range; sums are f32 in an order that depends on the extents only.  A NaN reaches the
+ * elements that it takes part in.  With a [M,K], b [K,N] and y = a . b, and each operand rounded
  * along the contraction it enters: y = (a along rows) (b along columns), ga = (gy along rows) (b along rows),
  * gb = (a along columns) (gy along columns).  A and B are 16-byte aligned, their scales 4-byte aligned; K is at most 2^28.
  * ws: ag_matmul_e4m3_f32_workspace() bytes, 16-byte aligned. */
@@ -432,7 +436,7 @@ ag_status_t ag_rms_norm_grad_f32(ag_stream_t stream, const float *h, const float
 
 /* clip[0] = sqrt(sum of the squares of all elements of `count` arrays), clip[1] = clip[0] <= max_norm ? 1 :
  * max_norm / clip[0]: two floats in device memory.  Squares are added in 64 bits in a fixed order.  A NaN among the
- * elements makes both NaN; an infinity makes the coefficient 0.  xs, ns: host tables, read before the call returns.  ws:
+ * elements makes both NaN; an infinity makes the coefficient 0 (1 if max_norm is infinite: nothing is clipped).  xs, ns: host tables, read before the call returns.  ws:
  * ag_global_norm_f32_workspace() bytes, 8-byte aligned. */
 size_t ag_global_norm_f32_workspace(int count, const size_t *ns);
 ag_status_t ag_global_norm_f32(ag_stream_t stream, int count, const float *const *xs, const size_t *ns, float max_norm,

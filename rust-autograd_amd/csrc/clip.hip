@@ -2,7 +2,7 @@
 //
 //   norm = sqrt(sum over arrays and elements of g^2)      coefficient = norm <= max_norm ? 1 : max_norm / norm
 //
-// A NaN anywhere gives a NaN coefficient, an infinity the coefficient 0.  The squares are added in 64 bits (no gradient
+// A NaN anywhere gives a NaN coefficient, an infinity the coefficient 0 (1 if max_norm is infinite).  The squares are added in 64 bits (no gradient
 // overflows them), each block over its own range and the blocks' sums in order, so a result does not depend on timing.
 #include <algorithm>
 #include <new>

@@ -58,7 +58,8 @@ __device__ inline unsigned finite_magnitude(quad_t v)
 
 // Biased exponent of the smallest power of two s >= 2^-117 with amax <= 448 s (448 = 1.75 * 2^8), from the bits of amax;
 // 1 for a block of zeros.  Integer arithmetic on the exponent field, so there is no rounding to disagree about.  (From 2^-117
-// on the smallest value of a block, 2^-9 of its scale, is a normal bf16 number.)
+// on the smallest value of a block, 2^-9 of its scale, is a normal bf16 number.  The largest block of f32 has byte 247; its
+// elements from 1.9375 * 2^127 on are rounded to 256 * 2^120, which is an infinity in bf16 and f32.)
 __device__ inline unsigned scale_byte(unsigned amax)
 {
     const int e = (int)(amax >> 23) - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);

@@ -29,7 +29,8 @@ struct GemmE4m3 {
     int splits, per_split;  // slices of the contraction and blocks of 128 in each; splits > 1: c is [splits][M][N]
 };
 
-// The factor that a scale byte stands for (bytes 1..254; 0 stands for 2^-127, which no block that this library rounds has).
+// A scale byte as the f32 whose exponent field it is.  The widening instruction reads that field alone: 0 is a factor of
+// 2^-127 there, 255 gives NaN.
 __device__ inline float scale_factor(unsigned word, int i) { return __uint_as_float(((word >> (8 * i)) & 0xffu) << 23); }
 
 // Eight consecutive e4m3 values times s, in bf16.

@@ -208,6 +208,33 @@ def test_output_rows_keep_what_lies_between_them(K, rng, m, n, k):
     assert (got[:, :n] == 0.0).all() and (got[:, n:] == 7.0).all()
 
 
+@pytest.mark.parametrize("m,n", [(1, 64), (30, 64), (200, 300), (1030, 3900), (2100, 4400)])
+def test_products_at_the_ends_of_the_scales(K, m, n):
+    """Every value that bf16 holds enters exactly, whatever the byte, and a smaller one rounded to nearest; from 1.9375 * 2^127 on an f32 is rounded to 2^128, which
+    counts as an infinity."""
+    def product(byte, value, power):
+        q, s = torch.zeros(m, 128, device="cuda"), torch.full((m, 4), 127, dtype=torch.uint8, device="cuda")
+        q[:, 5], s[:, 0] = value, byte
+        b = torch.zeros(n, 128, device="cuda")
+        b[:, 5] = 2.0 ** power
+        return K.matmul_e4m3(K.E4m3(q.to(torch.float8_e4m3fn), s.view(torch.float8_e8m0fnu), 128), K.quantize_e4m3(b))
+
+    for byte, value in ((0, 1.0), (1, 1.0), (1, 1.75 * 2.0 ** -6), (5, 2.0 ** -9), (9, 2.0 ** -9), (10, 2.0 ** -9), (10, 448.0), (247, 2.0 ** -9),
+                        (247, -240.0), (248, 1.0), (254, -1.875)):
+        power = -60 if byte > 127 else 60
+        # multiples of 2^-133 are what bf16 holds below 2^-126: 1.75 * 2^-6 * 2^-126 = 3.5 * 2^-133 lies between two of them
+        # and is rounded to the even one, 4 * 2^-133; every other value of the list is a multiple
+        held = np.round(value * 2.0 ** (byte - 127 + 133)) * 2.0 ** -133
+        assert held == (2.0 ** -131 if value == 1.75 * 2.0 ** -6 else value * 2.0 ** (byte - 127))
+        assert (product(byte, value, power) == held * 2.0 ** power).all(), (byte, value)
+    assert torch.isinf(product(254, 2.0, -60)).all() and torch.isnan(product(255, 1.0, -60)).all()
+    a, b = torch.zeros(m, 128, device="cuda"), torch.zeros(n, 128, device="cuda")
+    b[:, 0] = 2.0 ** -20
+    for value, want in ((1.9375 * 2.0 ** 127 * (1 - 2.0 ** -23), 1.875 * 2.0 ** 107), (1.9375 * 2.0 ** 127, np.inf), (-3.4028234e38, -np.inf)):
+        a[:, 0] = value
+        assert (K.quantize_matmul_e4m3(a, K.quantize_e4m3(b)) == want).all(), value
+
+
 def test_empty_extents(K):
     z = torch.zeros
     assert K.quantize_e4m3(z(0, 40, device="cuda")).q.shape == (0, 128)

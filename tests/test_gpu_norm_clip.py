@@ -410,3 +410,12 @@ def test_arrays_beyond_the_caches_have_the_bits_of_their_parts(K, rng, n):
     # (a block adds its rows in f32 in turn: at most all of them)
     assert ((gw.double() - sums).abs() <= (rows + 4) * U * sizes + TINY).all()
     torch.cuda.empty_cache()
+
+
+def test_nothing_is_clipped_to_an_infinite_norm(K):
+    x = torch.full((5000,), 2.0, device="cuda")
+    x[77] = float("inf")
+    for xs in ([x], [x] * 200):  # one block, several
+        outs, clip = K.clip_by_global_norm(xs, float("inf"))
+        assert torch.isinf(clip[0]) and clip[1] == 1 and all(torch.equal(o, x) for o in outs)
+    assert K.global_norm([x], 3.0e38)[1] == 0
