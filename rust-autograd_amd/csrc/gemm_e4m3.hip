@@ -65,11 +65,12 @@ __device__ inline const unsigned char *uniform(const unsigned char *p)
 // of 128 bytes, and a word of scales per row (four blocks, one of which the step uses).  The 16-byte piece c of row r stands
 // at place c ^ (r & 7) ^ ((r >> 3) & 1), so that 16 consecutive rows read at one piece fall on all 64 banks.
 //
-// What bounds it is power: with Gaussian operands the chip holds the matrix instruction alone, fed from registers, at
-// 1830 TFLOP/s (1.75 GHz; 2480 with zeros), and lowers its clock as the rest of the loop gets out of the way.  4096^3
-// takes 97 us (1415 TFLOP/s), 16384 x 8192 x 8192 1.44-1.46 ms (1500-1530; a bf16 product of the library, from operands
-// twice the size, 1.32 ms), the matrix unit busy for 83 % of the time.  What brought it there, at 4096^3 and at
-// 16384 x 8192 x 8192: every load of a step issued behind the barrier and operands widened where they are used 104 us,
+// What bounds it is power first: with Gaussian operands the chip holds the matrix instruction alone, fed from registers, at
+// 1830 TFLOP/s (1.75 GHz; 2480 with zeros), and lowers its clock as the rest of the loop gets out of the way; and the rest
+// of the loop: the matrix unit is busy for 83 % of the time at 1.70 GHz, in the library's bf16 product for 86 % at 1.78.
+// 4096^3 takes 97-104 us from run to run (1320-1415 TFLOP/s; the library's bf16 product, from operands twice the size,
+// 91-102), 16384 x 8192 x 8192 1.44-1.51 ms (1455-1530; 1.33).  What brought it there, the best of a run each at 4096^3
+// and at 16384 x 8192 x 8192: every load of a step issued behind the barrier and operands widened where they are used 104 us,
 // 1.61 ms; the next group's operands widened between the instructions of the current one, LDS read a chunk ahead and the
 // barrier in front of a step's last chunk 101 us, 1.48 ms; one basic block per step (no tests around the loads) and the
 // loads spread over four groups 97 us, 1.44 ms.  Four waves of 128 x 128 need a third less of LDS and widening but stand

@@ -72,8 +72,8 @@ __device__ inline void norm_write(const NormArgs &a, size_t row, long long i, qu
 // without streaming stores and loads, 15 with the half wave's maxima exchanged through LDS); one row of 4096 4.8 us.
 // Stores stream always (1024 x 4096: 9.7 and 12.5 us), loads from kStreamBytes on, beyond what the last-level cache keeps
 // between two kernels (4096 x 4096, whose arrays it does keep: 36 us without, 39 with; 16384 x 4096: 151 and 139).  The
-// quads of a thread come in small steps of the row's length: 16384 x 5001 to 8 bits 202 us with 5 quads a thread, 233
-// with 8; its gradient 251 and 336.
+// quads of a thread come in small steps of the row's length: 16384 x 5001 to 8 bits 197 us with 5 quads a thread, 232
+// with 8; its gradient, three quads a thread and four, 246 and 257.
 template <int T, int Q, bool STREAM>
 __global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_kernel(NormArgs a, unsigned rows)
 {
@@ -94,7 +94,8 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_kernel(NormArgs a,
         for (int k = 0; k < Q; ++k) h[k] += b[k];
     }
     // The weight stays in cache.  It is read ahead of the sum, so that one row alone does not wait twice (1 x 8192 4.9 us,
-    // behind it 5.7), but for the longest rows, whose registers it would spill (2048 x 32768 199 us, ahead 271).
+    // behind it 5.7), but for the longest rows, of which it would send dozens of registers to scratch (2048 x 32768 192 us,
+    // ahead 264; six go there all the same).
     constexpr bool LATE = T == 1024 && Q == 8;
     if (!LATE)
 #pragma unroll
@@ -187,7 +188,7 @@ __device__ inline quad_t grad_quad(quad_t h, quad_t w, quad_t g, quad_t gh, doub
 // A group of T threads walks rows in steps of the number of groups, with the row in registers and its share of gw beside
 // it: gw costs one [G][n] array of partial sums, folded in a fixed order below, instead of a second pass over gy and h.
 // T = 64: four groups share a block of 256 and add their sums through LDS at the end.  Bound by HBM: 16384 x 4096 with gh
-// 192 us, the fold included (5.6 TB/s; without streaming stores and loads 200).
+// 190 us, the fold included (5.7 TB/s; without streaming stores and loads 200).
 template <int T, int Q, bool STREAM>
 __global__ __launch_bounds__(T == 64 ? 256 : T) void rms_norm_grad_kernel(NormGradArgs a, unsigned rows)
 {
@@ -320,13 +321,12 @@ __global__ __launch_bounds__(kFoldGroups * 8) void rms_norm_grad_fold_kernel(con
 
 constexpr int kMaxRegisterRow = 4 * 8 * 1024;
 
-// Blocks that share the rows of a gradient: two per CU, at most one per row.
-// Rows of up to this many elements have a wave each in the gradient: 65536 x 512 takes 111 us, 200000 x 128 102, with a
-// block of 256 each 227 and 718.
+// Rows of up to this many elements have a wave each in the gradient: 65536 x 512 takes 69 us, 200000 x 128 59, with a
+// block of 256 each 194 and 672.
 constexpr int kWaveRow = 1024;
 
-// Blocks that share the rows of a gradient: two per CU (three: 8192 x 4096 208 us for both directions, two: 203), of one
-// row at a time or, where a wave has a row, four; not more than there are rows.
+// Blocks that share the rows of a gradient: two per CU with a row at a time (three: 8192 x 4096 208 us for both directions,
+// two: 203), eight per CU with four rows at a time where a wave has a row; no more than the rows fill.
 inline unsigned norm_grad_blocks(long long rows, int n)
 {
     const long long groups = n <= kWaveRow ? (rows + 3) / 4 : rows, most = (n <= kWaveRow ? 8LL : 2LL) * device_cus();
