@@ -553,17 +553,16 @@ def _here(t, name, dtype=torch.float32):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _ints(name, rows, n):
+def _ints(name, m, n, k=0):
     """Refuses extents that the C ABI's ints do not hold (ctypes would pass the low 32 bits)."""
-    if rows > 0x7FFFFFFF or n > 0x7FFFFFFF:
-        raise capi.InvalidDims(f"{name}: extents {rows} and {n} (at most 2147483647)")
+    if m > 0x7FFFFFFF or n > 0x7FFFFFFF or k > 0x7FFFFFFF:
+        raise capi.InvalidDims(f"{name}: an extent of {max(m, n, k)} (at most 2147483647)")
 
 
 def _matrix(x, name):
     x = _here(x, name)
     if x.dim() != 2:
         raise capi.IncompatibleShape(f"{name}: input must be 2D (got {list(x.shape)})")
-    _ints(name, *x.shape)
     return x
 
 
@@ -579,7 +578,6 @@ def _e4m3(e, name):
     q, scales = _here(e.q, name, torch.float8_e4m3fn), _here(e.scales, name, torch.float8_e8m0fnu)
     if q.dim() != 2 or q.shape[1] != -(-e.n // 128) * 128 or scales.shape != (q.shape[0], -(-e.n // 512) * 4):
         raise capi.IncompatibleShape(f"{name}: values {list(q.shape)} and scales {list(scales.shape)} are not those of rows of {e.n} elements")
-    _ints(name, q.shape[0], e.n)
     return q, scales, q.shape[0], e.n
 
 
@@ -587,6 +585,7 @@ def quantize_e4m3(x, transpose=False):
     """x [rows, cols] rounded to 8 bits along its rows; transpose=True: along its columns, as the transposed array."""
     x = _matrix(x, "quantize_e4m3")
     rows, cols = x.shape
+    _ints("quantize_e4m3", rows, cols)
     e = _e4m3_empty(cols, rows, x.device) if transpose else _e4m3_empty(rows, cols, x.device)
     q, s = e.q.data_ptr(), e.scales.data_ptr()
     out = (None, None, q, s) if transpose else (q, s, None, None)
@@ -598,6 +597,7 @@ def quantize_e4m3_both(x):
     """Both of quantize_e4m3's results from one pass over x: (along rows, transposed)."""
     x = _matrix(x, "quantize_e4m3")
     rows, cols = x.shape
+    _ints("quantize_e4m3", rows, cols)
     e, t = _e4m3_empty(rows, cols, x.device), _e4m3_empty(cols, rows, x.device)
     check(capi.lib().ag_quantize_e4m3_f32(_stream(), x.data_ptr(), cols, rows, cols, e.q.data_ptr(), e.scales.data_ptr(), t.q.data_ptr(),
                                           t.scales.data_ptr()))
@@ -612,6 +612,7 @@ def matmul_e4m3(a, b):
     qb, sb, n, kb = _e4m3(b, "matmul_e4m3")
     if k != kb:
         raise capi.IncompatibleShape(f"matmul_e4m3: contractions of {k} and {kb} elements")
+    _ints("matmul_e4m3", m, n, k)
     c = torch.empty((m, n), dtype=torch.float32, device=qa.device)
     L = capi.lib()
     nbytes = L.ag_matmul_e4m3_f32_workspace(m, n, k)
@@ -628,6 +629,7 @@ def quantize_matmul_e4m3(x, b):
     m, k = x.shape
     if k != kb:
         raise capi.IncompatibleShape(f"quantize_matmul_e4m3: contractions of {k} and {kb} elements")
+    _ints("quantize_matmul_e4m3", m, n, k)
     c = torch.empty((m, n), dtype=torch.float32, device=x.device)
     L = capi.lib()
     nbytes = L.ag_quantize_matmul_e4m3_f32_workspace(m, n, k)
