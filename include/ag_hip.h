@@ -400,7 +400,8 @@ ag_status_t ag_quantize_e4m3_f32(ag_stream_t stream, const float *x, int ldx, in
  * two elements is exact but for f32's range; sums are f32 in an order that depends on the extents only.  A NaN reaches the
  * elements that it takes part in.  With a [M,K], b [K,N] and y = a . b, and each operand rounded
  * along the contraction it enters: y = (a along rows) (b along columns), ga = (gy along rows) (b along rows),
- * gb = (a along columns) (gy along columns).  A and B are 16-byte aligned, their scales 4-byte aligned; K is at most 2^28.
+ * gb = (a along columns) (gy along columns).  A and B are 16-byte aligned, their scales 4-byte aligned; K is at most 2^28,
+ * M and N at most 2^31 - 513 (but N beside up to 16 rows of A), the tiles as many as a launch holds (AG_ERR_INVALID_DIMS).
  * ws: ag_matmul_e4m3_f32_workspace() bytes, 16-byte aligned. */
 size_t ag_matmul_e4m3_f32_workspace(int M, int N, int K);
 ag_status_t ag_matmul_e4m3_f32(ag_stream_t stream, int M, int N, int K, const uint8_t *A, const uint8_t *a_scales,
