@@ -437,8 +437,8 @@ ag_status_t ag_rms_norm_grad_f32(ag_stream_t stream, const float *h, const float
 
 /* clip[0] = sqrt(sum of the squares of all elements of `count` arrays), clip[1] = clip[0] <= max_norm ? 1 :
  * max_norm / clip[0]: two floats in device memory.  Squares are added in 64 bits in a fixed order.  A NaN among the
- * elements makes both NaN; an infinity makes the coefficient 0 (1 if max_norm is infinite: nothing is clipped).  xs, ns: host tables, read before the call returns.  ws:
- * ag_global_norm_f32_workspace() bytes, 8-byte aligned. */
+ * elements makes both NaN; an infinity makes the coefficient 0 (1 if max_norm is infinite: nothing is clipped).  xs, ns:
+ * host tables, read before the call returns.  ws: ag_global_norm_f32_workspace() bytes, 8-byte aligned. */
 size_t ag_global_norm_f32_workspace(int count, const size_t *ns);
 ag_status_t ag_global_norm_f32(ag_stream_t stream, int count, const float *const *xs, const size_t *ns, float max_norm,
                                float *clip, void *ws, size_t ws_bytes);

@@ -538,7 +538,7 @@ class E4m3(NamedTuple):
 
     def values(self):
         """The f32 values [rows, n] it stands for."""
-        power = (self.scales.view(torch.uint8).int() << 23).view(torch.float32)[:, : self.q.shape[1] // 128]
+        power = self.scales.float()[:, : self.q.shape[1] // 128]
         return (self.q.float().view(self.q.shape[0], -1, 128) * power[:, :, None]).view(self.q.shape)[:, : self.n]
 
 

@@ -351,3 +351,12 @@ def test_tiles_of_128_four_steps_deep(K, rng, k):
 def test_the_extents_of_these_tests_reach_every_form():
     reached = {form(m, n, k, cus()) for m, n, k in PRODUCTS} | {form(*a_tile_of_128_per_cu(), 768, cus())}
     assert reached == {(0, 16, False), (0, 32, False), (64, 4, False), (64, 4, True), (128, 4, False), (128, 2, False), (256, 2, False)}
+
+
+def test_values_of_an_operand_at_the_ends_of_the_scales(K):
+    """What values() says is what the product reads: byte 0 is 2^-127, 255 is NaN."""
+    q = torch.ones(7, 128, device="cuda")
+    scales = torch.tensor([0, 1, 10, 127, 247, 254, 255], dtype=torch.uint8, device="cuda")[:, None].expand(7, 4).contiguous()
+    got = host(K.E4m3(q.to(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu), 100).values())
+    want = np.exp2(np.array([0.0, 1, 10, 127, 247, 254, np.nan]) - 127)
+    assert got.shape == (7, 100) and np.array_equal(got, np.repeat(want[:, None], 100, axis=1), equal_nan=True)
